@@ -97,6 +97,12 @@ SIGNATURES = [
     ("e4b_k_attn_decode", _i32, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _u32, _f32,
                                  _i32, _vp, _vp]),
     ("e4b_k_attn_prefill", _i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _u32, _vp]),
+    ("e4b_kv_page_bytes", _sz, [_i32, _i32, _i32, _i32]),
+    ("e4b_kv_row", _i64, [_vp, _vp, _i64]),
+    ("e4b_k_kv_append", _i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _i32, _i64, _vp]),
+    ("e4b_k_kv_gather", _i32, [_vp, _vp, _vp, _vp, _vp]),
+    ("e4b_attn_paged_ws_bytes", _i32, [_vp, _vp, _i32, _i32, _i32, _i32, _P(_sz)]),
+    ("e4b_k_attn_paged", _i32, [_vp, _vp, _vp, _i32, _i64, _i32, _f32, _i32, _i32, _vp, _i64, _vp, _sz, _vp]),
     ("e4b_create", _vp, [_vp]),
     ("e4b_set_tensor", _i32, [_vp, C.c_char_p, _i32, _P(_i64), _i32, _vp, _sz]),
     ("e4b_finalize", _i32, [_vp]),
@@ -165,6 +171,35 @@ class MoeWeightsC(C.Structure):
         ("dense_gate_up", _vp), ("exp_gate_up", _vp), ("dense_down", _vp), ("exp_down", _vp),
         ("post_ffw1", _vp), ("post_ffw2", _vp), ("post_ffw", _vp),
     ]
+
+
+KV_F16 = 0
+KV_Q4 = 1
+PAGE_NONE = 0xFFFFFFFF
+PREP_V_RMS = 1
+PREP_V_IS_K = 2
+
+
+class PagedKvC(C.Structure):
+    """struct e4b_paged_kv (include/e4b.h)."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("type", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("page", _i32), ("n_pages", _i32), ("table_stride", _i32)]
+
+
+class KvBatchC(C.Structure):
+    """struct e4b_kv_batch (include/e4b.h)."""
+
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("n_seq", _i32), ("n_tok", _i32), ("max_q", _i32),
+                ("max_kv", _i32)]
+
+
+class HeadPrepC(C.Structure):
+    """struct e4b_head_prep (include/e4b.h)."""
+
+    _fields_ = [("q_norm", _vp), ("k_norm", _vp), ("inv_freq", _vp), ("rope_angles", _i32), ("eps", _f32),
+                ("flags", _u32)]
+
 
 for _name, _res, _args in SIGNATURES:
     _fn = getattr(lib, _name)

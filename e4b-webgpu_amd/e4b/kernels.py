@@ -9,7 +9,8 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import DT_F16, DT_F32, check, lib
+from ._lib import (DT_F16, DT_F32, KV_F16, KV_Q4, PREP_V_IS_K, PREP_V_RMS, HeadPrepC, KvBatchC, PagedKvC, check,
+                   lib)
 from .device import DeviceBuffer
 from .formats import q40_pack, q6k_pack
 
@@ -264,3 +265,97 @@ class MoeLayer:
         check(lib.e4b_k_router_top8(C.byref(self.w), _vp(self.h), _vp(self.idx), _vp(self.wts), None),
               "e4b_k_router_top8")
         return self.idx.download(np.uint32, 8), self.wts.download(np.float32, 8)
+
+
+def _addr(x) -> int | None:
+    return x.ptr if isinstance(x, DeviceBuffer) else x
+
+
+class KvBatch:
+    """The new tokens of several sequences (struct e4b_kv_batch): q_start
+    [n_seq + 1] and kv_len [n_seq], int32 on the device (DeviceBuffers or
+    addresses), kept by the caller; max_q and max_kv bound their lengths."""
+
+    def __init__(self, q_start, kv_len, n_seq: int, n_tok: int, max_q: int, max_kv: int):
+        self._keep = (q_start, kv_len)
+        self.n_tok = n_tok
+        self.c = KvBatchC(_addr(q_start), _addr(kv_len), n_seq, n_tok, max_q, max_kv)
+        self.ref = C.byref(self.c)
+
+    @classmethod
+    def from_lengths(cls, q_len, kv_len, n_tok: int | None = None) -> "KvBatch":
+        """From host lengths; n_tok > sum(q_len) is a padded batch."""
+        q_len, kv_len = np.asarray(q_len, np.int32), np.asarray(kv_len, np.int32)
+        start = np.concatenate([[0], np.cumsum(q_len)]).astype(np.int32)
+        return cls(DeviceBuffer.from_array(start), DeviceBuffer.from_array(kv_len), len(q_len),
+                   int(start[-1]) if n_tok is None else n_tok, max(int(q_len.max(initial=1)), 1),
+                   max(int(kv_len.max(initial=1)), 1))
+
+
+class HeadPrep:
+    """Head norms and rotation of appended rows (struct e4b_head_prep); the
+    vectors are f32 on the device, None = no norm."""
+
+    def __init__(self, q_norm, k_norm, inv_freq, rope_angles: int, eps: float = 1e-6, v_rms: bool = True,
+                 v_is_k: bool = False):
+        self._keep = (q_norm, k_norm, inv_freq)
+        self.v_is_k = v_is_k
+        self.c = HeadPrepC(_addr(q_norm), _addr(k_norm), _addr(inv_freq), rope_angles, eps,
+                           (PREP_V_RMS if v_rms else 0) | (PREP_V_IS_K if v_is_k else 0))
+        self.ref = C.byref(self.c)
+
+
+class PagedKV:
+    """A paged key/value cache (struct e4b_paged_kv): pools of n_pages pages
+    and the table [n_seq][table_stride] of each sequence's pages.  kind: "f16"
+    or "q4".  Pools and table are the caller's (k, v, table: DeviceBuffers or
+    addresses), or are allocated here (n_seq table rows, all E4B_PAGE_NONE)."""
+
+    def __init__(self, kind: str, kv_heads: int, head_dim: int, page: int, n_pages: int, table_stride: int, k=None,
+                 v=None, table=None, n_seq: int = 0):
+        self.type = {"f16": KV_F16, "q4": KV_Q4}[kind]
+        self.kvh, self.hd, self.page, self.n_pages, self.stride = kv_heads, head_dim, page, n_pages, table_stride
+        self.page_bytes = lib.e4b_kv_page_bytes(self.type, kv_heads, head_dim, page)
+        if not self.page_bytes:
+            check(-1, "e4b_kv_page_bytes")
+        if (k is None) != (v is None):
+            raise ValueError("both pools are the caller's, or neither")
+        if k is None:
+            k, v = DeviceBuffer(n_pages * self.page_bytes), DeviceBuffer(n_pages * self.page_bytes)
+        if table is None:
+            table = DeviceBuffer(max(n_seq, 1) * table_stride * 4)
+            table.fill(0xFF)
+        self.k, self.v, self.table = k, v, table
+        self.c = PagedKvC(_addr(k), _addr(v), _addr(table), self.type, kv_heads, head_dim, page, n_pages,
+                          table_stride)
+        self.ref = C.byref(self.c)
+
+    def append_dev(self, batch: KvBatch, prep: HeadPrep, qkv, dtype: int, q_heads: int, q_out=None,
+                   q_dtype: int = DT_F32, stride: int | None = None, q_stride: int | None = None,
+                   stream=None) -> None:
+        """Norms, rotation and rows of the batch's tokens (e4b_k_kv_append); strides default to rows one behind the other."""
+        if stride is None:
+            stride = (q_heads + (1 if prep.v_is_k else 2) * self.kvh) * self.hd
+        check(lib.e4b_k_kv_append(self.ref, batch.ref, prep.ref, _addr(qkv), dtype, stride, q_heads, _addr(q_out),
+                                  q_dtype, q_heads * self.hd if q_stride is None else q_stride, stream),
+              "e4b_k_kv_append")
+
+    def gather_dev(self, batch: KvBatch, k_out, v_out, stream=None) -> None:
+        """The batch's rows as f16 [n_tok][kv_heads][head_dim] (e4b_k_kv_gather)."""
+        check(lib.e4b_k_kv_gather(self.ref, batch.ref, _addr(k_out), _addr(v_out), stream), "e4b_k_kv_gather")
+
+    def attn_ws_bytes(self, batch: KvBatch, q_dtype: int, q_heads: int, window: int = 0, sinks: int = 0) -> int:
+        """Scratch of such an attn_dev call (e4b_attn_paged_ws_bytes)."""
+        n = C.c_size_t(0)
+        check(lib.e4b_attn_paged_ws_bytes(self.ref, batch.ref, q_dtype, q_heads, window, sinks, C.byref(n)),
+              "e4b_attn_paged_ws_bytes")
+        return n.value
+
+    def attn_dev(self, batch: KvBatch, q, q_dtype: int, q_heads: int, out, window: int = 0, sinks: int = 0,
+                 scale: float = 1.0, q_stride: int | None = None, out_stride: int | None = None, ws=None,
+                 ws_bytes: int = 0, stream=None) -> None:
+        """Attention of the batch's queries over the cache (e4b_k_attn_paged)."""
+        n = q_heads * self.hd
+        check(lib.e4b_k_attn_paged(self.ref, batch.ref, _addr(q), q_dtype, n if q_stride is None else q_stride,
+                                   q_heads, scale, window, sinks, _addr(out), n if out_stride is None else out_stride,
+                                   _addr(ws), ws_bytes, stream), "e4b_k_attn_paged")

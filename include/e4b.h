@@ -271,6 +271,121 @@ int e4b_k_attn_prefill(const float* q, const void* kc, const void* vc, void* out
                        int slots, int window, uint32_t p0, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged key/value cache: many sequences at once, each of a length of its own,
+ * in pages of a shared pool, as f16 or in 4 bits.  No counterpart in the
+ * reference (one sequence, one ring per layer): this is what serving several
+ * conversations needs beside e4b_k_attn_decode / e4b_k_attn_prefill.
+ *
+ * Per pool (K and V) and page: [kv_heads] blocks of `page` rows.
+ *   E4B_KV_F16  a block is f16 [page][head_dim]
+ *   E4B_KV_Q4   a block is codes [page][head_dim / 2 bytes], then f16 scales
+ *               [page][head_dim / 32]: value = (code - 8) * scale per 32 dims.
+ *               Dword w of a row's codes holds dims 8w .. 8w + 7, dims 0..7 at
+ *               bits 0, 16, 8, 24, 4, 20, 12, 28 (the order of e4b_q40_pack).
+ *               Scales have at most 8 significant bits, so every value is
+ *               exact in f16.  Attention takes any f16 scales; values of other
+ *               ones are rounded to f16.
+ * Position p of a sequence is row p % page of page table[p / page] of its row
+ * of the table; an entry >= n_pages (E4B_PAGE_NONE) is no page: reads find
+ * nothing there and appends write nothing.  Pages that no visible position
+ * needs (behind a window) may be given back and their entries changed.  One
+ * page may stand in several sequences' rows (a shared prefix) as long as no
+ * call appends to it; no two tokens of one call may have the same row.
+ *
+ * Batch: tokens q_start[i] .. q_start[i + 1] - 1 are the newest ones of
+ * sequence i, at positions kv_len[i] - q_len .. kv_len[i] - 1, with q_len =
+ * q_start[i + 1] - q_start[i] >= 0 and kv_len counting them.  Both arrays and
+ * the table are device memory, read by the kernels: a captured call replays
+ * with what they hold then.  Tokens behind q_start[n_seq] (a padded batch) are
+ * left as they are, in every output; so are q_out rows of tokens at negative
+ * positions (kv_len < q_len).  n_seq or n_tok of 0 is a call that does
+ * nothing.  max_q and max_kv are host bounds of q_len and kv_len; they choose
+ * the kernels and the split of the work.  Tokens of a sequence with more than
+ * max_q of them may be left out; kv_len may exceed max_kv, at some cost in
+ * time.
+ * ------------------------------------------------------------------------- */
+#define E4B_KV_F16 0
+#define E4B_KV_Q4 1
+#define E4B_PAGE_NONE 0xffffffffu
+
+typedef struct e4b_paged_kv {
+  void* k;                /* pools: n_pages of e4b_kv_page_bytes each, 16-byte aligned */
+  void* v;
+  const uint32_t* table;  /* [n_seq][table_stride] pages of each sequence */
+  int32_t type;           /* E4B_KV_* */
+  int32_t kv_heads;       /* 1 .. 256 */
+  int32_t head_dim;       /* 128, 256 or 512 */
+  int32_t page;           /* positions per page: 16, 32, 64, 128 or 256 */
+  int32_t n_pages;
+  int32_t table_stride;   /* entries of a table row */
+} e4b_paged_kv;
+
+typedef struct e4b_kv_batch {
+  const int32_t* q_start; /* [n_seq + 1], not falling; q_start[0] = 0 unless tokens before are to be skipped */
+  const int32_t* kv_len;  /* [n_seq] */
+  int32_t n_seq;          /* <= 65535 */
+  int32_t n_tok;          /* token rows of the buffers, >= q_start[n_seq], <= 2^24 */
+  int32_t max_q;
+  int32_t max_kv;
+} e4b_kv_batch;
+
+#define E4B_PREP_V_RMS 1u   /* v heads get a scale-less RMS */
+#define E4B_PREP_V_IS_K 2u  /* the rows hold no v heads: v is the raw k head (full layers with V = K) */
+typedef struct e4b_head_prep {
+  const float* q_norm;    /* [head_dim] head-RMS weights, 16-byte aligned; NULL: q is not normed */
+  const float* k_norm;    /* likewise of k */
+  const float* inv_freq;  /* [rope_angles] (e4b_rope_inv_freq) */
+  int32_t rope_angles;    /* rotated pairs (d, d + head_dim / 2), d < rope_angles <= head_dim / 2 */
+  float eps;
+  uint32_t flags;         /* E4B_PREP_* */
+} e4b_head_prep;
+
+/* bytes of one page of one pool, 0 for a cache that is not supported */
+size_t e4b_kv_page_bytes(int type, int kv_heads, int head_dim, int page);
+/* Host only: the row of head 0 that holds position `pos` of a sequence whose
+ * table row `table_row` (host memory) is; head g's is g * page rows further, a
+ * row being the pool's unit of one position and head.  E4B_ERANGE where the
+ * position has no page.  kv's pointers are not used. */
+int64_t e4b_kv_row(const e4b_paged_kv* kv, const uint32_t* table_row, int64_t pos);
+
+/* Appends the batch's tokens: rows [q heads | k heads | v heads] of head_dim
+ * (dtype E4B_DT_F32 or E4B_DT_F16, `stride` elements apart) become
+ *   q_out = rope(rms(q) q_norm)   (q_dtype f32 or f16, rows q_stride apart; NULL: not wanted)
+ *   K row = rope(rms(k) k_norm),  V row = rms(v) or v
+ * at their positions.  q_out may be qkv itself, with the same type and stride.
+ * 4 bits, per 32 dims: a = the value of largest magnitude (the first of
+ * several), scale = a / -8 rounded to 8 significant bits (at most 8160 in
+ * magnitude), code = x / scale rounded to even, + 8, cut to 0..15; a block
+ * with a value that is not finite reads as NaN.  q_heads may be 0. */
+int e4b_k_kv_append(const e4b_paged_kv* kv, const e4b_kv_batch* batch, const e4b_head_prep* prep, const void* qkv,
+                    int dtype, int64_t stride, int q_heads, void* q_out, int q_dtype, int64_t q_stride,
+                    void* stream);
+
+/* The batch's rows of the cache as f16 [n_tok][kv_heads][head_dim] (either
+ * output may be NULL); rows of positions without a page are zero.  With
+ * q_len = kv_len it reads whole sequences. */
+int e4b_k_kv_gather(const e4b_paged_kv* kv, const e4b_kv_batch* batch, void* k_out, void* v_out, void* stream);
+
+/* Scratch that e4b_k_attn_paged needs for such a call (the sizes, the types
+ * and max_q / max_kv count, not the pointers), >= 0 bytes. */
+int e4b_attn_paged_ws_bytes(const e4b_paged_kv* kv, const e4b_kv_batch* batch, int q_dtype, int q_heads, int window,
+                            int sinks, size_t* bytes);
+
+/* Attention of the batch's queries (prepped, f32 or f16, rows q_stride apart)
+ * over the cache that holds their keys:
+ *   out[t][h] = sum_k softmax_k(scale q.k) v_k   (f16, rows out_stride apart)
+ * over the keys k <= p of the token's position p with k > p - window or
+ * k < sinks (window 0: all of them); KV head h / (q_heads / kv_heads).  A
+ * token that sees no key gets zeros.  What masked, absent or unused rows hold
+ * does not matter, infinities and NaN included.
+ * ws: scratch of e4b_attn_paged_ws_bytes bytes, 16-byte aligned, for this call
+ * alone until it has run; NULL: the library's workspace (calls on one device
+ * that use it must be ordered; see "Workspace" above). */
+int e4b_k_attn_paged(const e4b_paged_kv* kv, const e4b_kv_batch* batch, const void* q, int q_dtype, int64_t q_stride,
+                     int q_heads, float scale, int window, int sinks, void* out_f16, int64_t out_stride, void* ws,
+                     size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Engine: the per-token batch-1 decode step of an E4B-shaped decoder
  * (35 layers, 4 sliding : 1 global, GeGLU FFN, per-layer embeddings, q4_0
  * linears, Q6_K tied embedding / lm-head, f16 KV ring).  Replaces the engine
