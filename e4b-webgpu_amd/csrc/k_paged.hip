@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs A) {
   const SeqSpan s = seq_span(P, i);
   const int pos = s.p0 + (t - s.q0);
   if (pos < 0 || t < s.q0 || t - s.q0 >= s.n) return;
-  const int pg = paged_page(P.table + (int64_t)i * P.table_stride, P.table_stride, P.page_shift, P.n_pages, pos);
+  const int pg = paged_page(table_row(P, i), P.table_stride, P.page_shift, P.n_pages, pos);
   const int row = pos & ((1 << P.page_shift) - 1);
   const int heads = A.qh + (A.v_is_k ? 1 : 2) * P.kvh;
   auto put = [&](uint8_t* pool, int g, const T(&x)[E]) {
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void k_kv_gather(PagedArgs P, uint16_t* __rest
   const SeqSpan s = seq_span(P, i);
   if (t < s.q0 || t - s.q0 >= s.n) return;
   const int pos = s.p0 + (t - s.q0);
-  const int pg = paged_page(P.table + (int64_t)i * P.table_stride, P.table_stride, P.page_shift, P.n_pages, pos);
+  const int pg = paged_page(table_row(P, i), P.table_stride, P.page_shift, P.n_pages, pos);
   const int row = pos & ((1 << P.page_shift) - 1);
   for (int j = blockIdx.y * 4 + wave; j < 2 * P.kvh; j += 4 * gridDim.y) {
     const int g = j >> 1;

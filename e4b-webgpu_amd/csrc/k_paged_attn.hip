@@ -43,7 +43,7 @@ __global__ __launch_bounds__(64) void k_attn_paged(PagedAttnArgs A) {
   const int first = A.window > 0 ? max(0, pos - A.window + 1) : 0;
   for (int p = 0; p <= pos; ++p) {
     if (p < first && p >= A.sinks) p = first;
-    const int pg = paged_page(P.table + (int64_t)i * P.table_stride, P.table_stride, P.page_shift, P.n_pages, p);
+    const int pg = paged_page(table_row(P, i), P.table_stride, P.page_shift, P.n_pages, p);
     if (pg < 0) continue;
     const int64_t block = paged_block<Q4, HD>(P, pg, g);
     const int r = p & ((1 << P.page_shift) - 1);
@@ -82,5 +82,6 @@ int attn_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
 }  // namespace
 
 int launch_attn_paged(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st) {
+  if (a.max_rows <= kPagedFewRows) return launch_attn_paged_few(a, hd, q4, q16, st);
   return hd == 128 ? attn_hd<128>(a, q4, q16, st) : hd == 256 ? attn_hd<256>(a, q4, q16, st) : attn_hd<512>(a, q4, q16, st);
 }

@@ -26,7 +26,8 @@ E4B_HD int paged_row_bytes(bool q4, int hd) { return q4 ? hd / 2 + hd / 16 : 2 *
 
 // The page that holds position p of a sequence with table row `row`, or -1:
 // before the sequence, past the table, or an entry that names no page.
-E4B_HD int paged_page(const uint32_t* row, int table_stride, int page_shift, int n_pages, int64_t p) {
+template <typename Table>
+E4B_HD int paged_page(Table row, int table_stride, int page_shift, int n_pages, int64_t p) {
   if (p < 0) return -1;
   const int64_t b = p >> page_shift;
   if (b >= table_stride) return -1;
@@ -50,12 +51,20 @@ struct PagedArgs {
 struct SeqSpan {
   int q0, n, p0, kv;
 };
+// The arrays are read with an index that is the same for all lanes and not
+// written while a kernel runs: through the scalar cache.
+typedef const __attribute__((address_space(4))) uint32_t* table_ptr;
+typedef const __attribute__((address_space(4))) int32_t* lens_ptr;
+DEV table_ptr table_row(const PagedArgs& P, int i) {
+  return (table_ptr)(uintptr_t)P.table + (int64_t)i * P.table_stride;
+}
 DEV SeqSpan seq_span(const PagedArgs& P, int i) {
   SeqSpan s;
-  const int a = P.q_start[i], b = P.q_start[i + 1];
+  const lens_ptr q_start = (lens_ptr)(uintptr_t)P.q_start, kv_len = (lens_ptr)(uintptr_t)P.kv_len;
+  const int a = q_start[i], b = q_start[i + 1];
   s.q0 = min(max(a, 0), P.n_tok);
   s.n = min(max(b, s.q0), P.n_tok) - s.q0;
-  s.kv = max(P.kv_len[i], 0);
+  s.kv = max(kv_len[i], 0);
   s.p0 = s.kv - s.n;
   return s;
 }
@@ -92,6 +101,7 @@ struct KvAppendArgs {
 int launch_kv_append(const KvAppendArgs& a, int hd, bool q4, bool x16, hipStream_t st);
 int launch_kv_gather(const PagedArgs& P, int hd, bool q4, uint16_t* k_out, uint16_t* v_out, hipStream_t st);
 
+constexpr int kPagedMaxSplits = 256;
 struct PagedAttnArgs {
   PagedArgs P;
   const void* q;            // f32 or f16 rows of qh heads
@@ -100,6 +110,17 @@ struct PagedAttnArgs {
   int64_t out_stride;
   int qh, gqa, window, sinks;
   float scale;
+  int max_q, max_kv;        // bounds of a sequence's tokens (<= n_tok) and positions
+  // the plan: rows (tokens x heads of a group) that a sequence has at most,
+  // blocks of them, splits of the keys, and where the splits' results go
+  int max_rows, nrb, ns;
+  size_t part_floats, ml_floats;
+  float* part;
+  float* part_ml;
 };
+// a few query rows per sequence and KV head (k_paged_decode.hip)
+void plan_attn_paged_few(PagedAttnArgs& a, int hd);
+int launch_attn_paged_few(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
+constexpr int kPagedFewRows = 16;  // most rows of a sequence and KV head that k_paged_decode.hip takes
 int launch_attn_paged(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
 #endif

@@ -1,5 +1,7 @@
 // paged.hip -- the C entry points of the paged key/value cache: argument
 // checks and launches (kernels: k_paged*.hip).
+#include <algorithm>
+
 #include "../../include/e4b.h"
 #include "paged.h"
 #include "util.h"
@@ -128,6 +130,11 @@ extern "C" int e4b_k_kv_gather(const e4b_paged_kv* kv, const e4b_kv_batch* batch
                           (hipStream_t)stream);
 }
 
+// splits' outputs, then their maxima and sums
+static size_t scratch_bytes(const PagedAttnArgs& a) {
+  return E4B_ALIGN256(a.part_floats * sizeof(float)) + a.ml_floats * sizeof(float);
+}
+
 // the checks of an attention call; *a is complete but for its pointers
 static int attn_setup(const char* fn, const e4b_paged_kv* kv, const e4b_kv_batch* batch, int q_dtype, int q_heads,
                       int window, int sinks, PagedAttnArgs* a, bool* empty) {
@@ -142,6 +149,13 @@ static int attn_setup(const char* fn, const e4b_paged_kv* kv, const e4b_kv_batch
   a->gqa = q_heads / kv->kv_heads;
   a->window = window;
   a->sinks = window ? sinks : 0;
+  a->ns = 1;
+  a->part_floats = a->ml_floats = 0;
+  if (*empty) return E4B_OK;
+  a->max_q = std::min(batch->max_q, batch->n_tok);
+  a->max_kv = batch->max_kv;
+  a->max_rows = (int)std::min<int64_t>((int64_t)a->max_q * a->gqa, 1 << 30);
+  if (a->max_rows <= kPagedFewRows) plan_attn_paged_few(*a, kv->head_dim);
   return E4B_OK;
 }
 
@@ -153,7 +167,7 @@ extern "C" int e4b_attn_paged_ws_bytes(const e4b_paged_kv* kv, const e4b_kv_batc
   bool empty;
   int rc = attn_setup(fn, kv, batch, q_dtype, q_heads, window, sinks, &a, &empty);
   if (rc) return rc;
-  *bytes = 0;
+  *bytes = scratch_bytes(a);
   return E4B_OK;
 }
 
@@ -169,8 +183,17 @@ extern "C" int e4b_k_attn_paged(const e4b_paged_kv* kv, const e4b_kv_batch* batc
   if (empty) return E4B_OK;
   if ((rc = check_rows(fn, "q", q, q_dtype, q_stride, q_heads, kv->head_dim))) return rc;
   if ((rc = check_rows(fn, "out", out_f16, E4B_DT_F16, out_stride, q_heads, kv->head_dim))) return rc;
-  (void)ws;
-  (void)ws_bytes;
+  if (const size_t need = scratch_bytes(a)) {
+    if (ws && (ws_bytes < need || !aligned(ws, 16)))
+      return e4b_fail(E4B_EINVAL, "%s: %zu bytes of scratch where %zu, 16-byte aligned, are needed", fn, ws_bytes, need);
+    if (!ws) {
+      Workspace w;
+      if ((rc = e4b_workspace(need, &w, (hipStream_t)stream))) return rc;
+      ws = w.buf;
+    }
+    a.part = (float*)ws;
+    a.part_ml = (float*)((uint8_t*)ws + E4B_ALIGN256(a.part_floats * sizeof(float)));
+  }
   a.q = q;
   a.q_stride = q_stride;
   a.out = (uint16_t*)out_f16;

@@ -1,0 +1,72 @@
+// paged_attn.h -- what the attention kernels over the paged cache share: the
+// tiles that a set of queries sees, and fragments of 4-bit rows as f16.
+#pragma once
+#include "paged.h"
+
+#ifdef __HIPCC__
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+constexpr int kPT = 32;  // keys per tile: two 16-key halves, each inside one page
+
+// Tiles of the keys that queries at positions p0 .. p1 see, in the order of
+// the keys: `sink` tiles from 0 on, then the ones from `from` on.
+struct TileRange {
+  int sink, from, n;
+  DEV int base(int t) const { return (t < sink ? t : t - sink + from) * kPT; }
+};
+DEV TileRange tile_range(int p0, int p1, int window, int sinks, int cap) {
+  const int first = window > 0 ? max(0, p0 - window + 1) : 0;
+  const int last = min(p1, cap - 1);
+  TileRange r;
+  r.from = first / kPT;
+  r.sink = min((min(sinks, first) + kPT - 1) / kPT, r.from);
+  r.n = last < 0 ? 0 : min(r.sink, last / kPT + 1) + max(0, last / kPT - r.from + 1);
+  return r;
+}
+// positions that the table has entries for
+DEV int paged_cap(const PagedArgs& P) {
+  return (int)min((int64_t)P.table_stride << P.page_shift, (int64_t)0x7fffffff);
+}
+DEV bool key_seen(int key, int pos, int window, int sinks) {
+  return key <= pos && (window == 0 || key > pos - window || key < sinks);
+}
+
+// eight codes of a dword as f16 values (code - 8) d, dims in order; d2 = (d, d).
+// A half 0x6400 | n is 1024 + n, one with n four bits up 1024 + 16 n: taking
+// 1032 off, or 1/16 of it less 72, is exact.
+DEV void q4_pairs(uint32_t w, h2v (&p)[4]) {
+  const uint32_t w8 = w >> 8, one = 0x64006400u, lo = 0x000F000Fu, hi = 0x00F000F0u;
+  const h2v c = {(_Float16)1032.f, (_Float16)1032.f}, s = {(_Float16)0.0625f, (_Float16)0.0625f},
+            e = {(_Float16)72.f, (_Float16)72.f};
+  p[0] = __builtin_bit_cast(h2v, (w & lo) | one) - c;
+  p[1] = __builtin_bit_cast(h2v, (w8 & lo) | one) - c;
+  p[2] = __builtin_elementwise_fma(__builtin_bit_cast(h2v, (w & hi) | one), s, -e);
+  p[3] = __builtin_elementwise_fma(__builtin_bit_cast(h2v, (w8 & hi) | one), s, -e);
+}
+DEV h2v h2_of(uint32_t w) { return __builtin_bit_cast(h2v, w); }
+DEV uint32_t u_of(h2v v) { return __builtin_bit_cast(uint32_t, v); }
+DEV h8v q4_frag(uint32_t w, h2v d2) {
+  h2v p[4];
+  q4_pairs(w, p);
+  return __builtin_bit_cast(h8v, make_uint4(u_of(p[0] * d2), u_of(p[1] * d2), u_of(p[2] * d2), u_of(p[3] * d2)));
+}
+// halves 0 or 1 of two dwords side by side
+DEV uint32_t lo_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+DEV uint32_t hi_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48
+DEV float quad_max4(float v) {
+  float t = v;
+  swapx32(v, t);
+  v = fmaxf(v, t);
+  t = v;
+  swapx16(v, t);
+  return fmaxf(v, t);
+}
+DEV float quad_sum4(float v) { return xsum_step<16>(xsum_step<32>(v)); }
+DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr float kNone = -3.0e38f;  // the running maximum before the first key
+#endif
