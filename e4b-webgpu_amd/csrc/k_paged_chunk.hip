@@ -1,0 +1,529 @@
+// k_paged_chunk.hip -- attention of many query rows per KV head over the paged
+// cache: prompts and their chunks (paged.h; a few rows: k_paged_decode.hip).
+//
+// Workgroup (tile of query rows of one sequence, KV head, split of the keys);
+// a row is (token, head of the group), token major, so the heads that share
+// K and V share a tile.  Key tiles of 32 are staged in LDS as f16, one tile
+// ahead, in two buffers; each wave has F fragments of 16 columns, a fragment
+// being 16 rows of f16 queries or 8 rows of f32 ones (high and low parts side
+// by side, as in k_paged_decode.hip):
+//   S^T (16 keys x 16 columns) = K . Q^T, K read row by row;
+//   O^T (16 dims x 16 columns) += V^T . P^T, V^T read with the transposing
+//   ds_read_b64_tr_b16, P as it lies in the registers after the softmax.
+// A fragment of K or V (1 KB of LDS reads) feeds F products: with F = 2 the
+// LDS's 128 bytes a clock and the matrix units' rate are matched.
+#include <algorithm>
+
+#include "../../include/e4b.h"
+#include "paged_attn.h"
+#include "util.h"
+
+namespace {
+
+typedef __fp16 tr4 __attribute__((__vector_size__(8)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) tr4 lds_tr4;
+
+// head dim 512: one fragment (its output alone is 128 registers) and 8 waves,
+// as LDS holds one workgroup's tiles
+template <int HD>
+constexpr int kFrags = HD == 512 ? 1 : 2;
+template <int HD>
+constexpr int kChunkWaves = HD == 512 ? 8 : 4;
+template <int HD, bool Q16>
+constexpr int kTileRows = kChunkWaves<HD> * kFrags<HD> * (Q16 ? 16 : 8);
+
+// The sequence and its tile that tile number `at` of the whole batch is; the
+// sequences that k_paged_decode.hip takes have none.  Later tiles first: they
+// see the most keys.
+struct TileAt {
+  int seq, tile;
+};
+DEV TileAt find_tile(const PagedAttnArgs& A, int rows_per, int at) {
+  const int lane = threadIdx.x & 63;
+  for (int b = 0; b < A.P.n_seq; b += 64) {
+    int n = 0;
+    if (b + lane < A.P.n_seq) {
+      const int q0 = min(max(A.P.q_start[b + lane], 0), A.P.n_tok);
+      const int rows = (min(max(A.P.q_start[b + lane + 1], q0), A.P.n_tok) - q0) * A.gqa;
+      n = rows <= A.few_rows ? 0 : (rows + rows_per - 1) / rows_per;
+    }
+    int upto = n;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int x = __shfl_up(upto, m, 64);
+      if (lane >= m) upto += x;
+    }
+    const uint64_t past = __ballot(at < upto);
+    if (past) {
+      const int f = __builtin_ctzll(past);
+      const int last = __builtin_amdgcn_readlane(upto, f) - 1 - at;
+      return {b + f, last};
+    }
+    at -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {-1, 0};
+}
+
+constexpr int kMinTiles = 8;  // key tiles of a split at least
+DEV int chunk_per(int n, int ns) { return max(kMinTiles, uni((n + ns - 1) / ns)); }
+
+// whether one of two f16 values is not finite
+DEV bool not_finite(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
+// dim d of a row
+template <int HD, bool Q4>
+DEV float cache_value(const uint8_t* block, int row, int d, int page_shift) {
+  if constexpr (Q4) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(block + row * (HD / 2) + d / 8 * 4);
+    const int pr = d % 8 / 2;
+    const int n = (int)(w >> (((pr & 1) << 3) + ((pr & 2) << 1) + 16 * (d & 1)) & 15) - 8;
+    return n * h2f(*reinterpret_cast<const uint16_t*>(block + (HD / 2 << page_shift) + row * (HD / 16) + d / 32 * 2));
+  } else {
+    return h2f(reinterpret_cast<const uint16_t*>(block)[row * HD + d]);
+  }
+}
+
+// 16-byte piece `p` of row r of a tile in LDS: rows are whole bank rounds
+// apart, so the pieces are moved by the row (K: 16 rows are read at once, V:
+// 16 rows of 32 bytes)
+template <int HD>
+DEV int k_piece(int r, int p) { return p ^ (r & 15); }
+template <int HD>
+DEV int v_piece(int r, int p) { return p ^ ((r & (HD == 128 ? 7 : 15)) << 1); }
+
+template <int HD, bool Q4, bool Q16>
+__global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(PagedAttnArgs A) {
+  constexpr int F = kFrags<HD>, NW = kChunkWaves<HD>, BM = kTileRows<HD, Q16>, RF = Q16 ? 16 : 8;
+  constexpr int QS = HD / 32, DT = HD / 16, KP = HD / 8, TP = kPT * KP;  // TP: 16-byte pieces of a K or V tile
+  __shared__ __align__(16) uint4 bufs[2][2 * TP];
+  const PagedArgs& P = A.P;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g4 = lane >> 4;
+  const int sp = blockIdx.x % A.ns, g = blockIdx.x / A.ns % P.kvh, at = blockIdx.x / A.ns / P.kvh;
+  const TileAt ta = find_tile(A, BM, at);
+  const int i = __builtin_amdgcn_readfirstlane(ta.seq), qt = __builtin_amdgcn_readfirstlane(ta.tile);
+  if (i < 0) return;
+  const SeqSpan s = seq_span(P, i);
+  const int rows = s.n * A.gqa;
+  const int t0 = qt * BM, t1 = min(t0 + BM, rows);  // rows of the tile
+  const int cap = paged_cap(P);
+  const int pa = s.p0 + uni(t0 / A.gqa), pb = s.p0 + uni((t1 - 1) / A.gqa);  // their positions
+  const TileRange R = tile_range(pa, pb, A.window, A.sinks, cap);
+  const int per = chunk_per(R.n, A.ns), live = uni((R.n + per - 1) / per);  // tiles of a split, splits that have any
+  const int n_tiles = max(0, min(per, R.n - sp * per)), first = sp * per;
+  if (n_tiles == 0 && !(sp == 0 && R.n == 0)) return;
+  const table_ptr trow = table_row(P, i);
+
+  // this wave's rows, and this lane's column of each fragment
+  const int w0 = t0 + wave * F * RF, w1 = min(w0 + F * RF, t1);
+  const bool any = w0 < t1;
+  const int wp0 = s.p0 + uni(min(w0, rows - 1) / A.gqa), wp1 = s.p0 + uni((max(w1, 1) - 1) / A.gqa);
+  int tok[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) tok[f] = min(w0 + f * RF + (c & (RF - 1)), rows - 1) / A.gqa;
+  // the column's row: whether there is one, and its head
+  auto row_of = [&](int f, bool& have) {
+    const int r = w0 + f * RF + (c & (RF - 1)), rc = min(r, rows - 1);
+    have = r < t1;
+    return g * A.gqa + rc - rc / A.gqa * A.gqa;
+  };
+
+  // ---- staging ----
+  struct Half {  // 16 keys: their page's blocks and the first row there
+    const uint8_t *k, *v;
+    int row;
+    bool there;
+  };
+  auto half_at = [&](int kb, int u) {
+    const int p = kb + 16 * u, b = p >> P.page_shift;
+    const uint32_t pg = trow[min(b, P.table_stride - 1)];
+    const bool there = b < P.table_stride && pg < (uint32_t)P.n_pages;
+    const int64_t blk = paged_block<Q4, HD>(P, there ? (int)pg : 0, g);
+    return Half{P.k + blk, P.v + blk, p & ((1 << P.page_shift) - 1), there};
+  };
+  // f16: rows go straight into LDS, 1 KB a wave at a time
+  constexpr int RI = 1024 / (2 * HD);             // rows of a copy
+  constexpr int HC = 16 / RI / NW;                // copies of a wave for a half of K or V
+  static_assert(HC * NW * RI == 16, "the waves share a half evenly");
+  int at_k[HC], at_v[HC];
+#pragma unroll
+  for (int j = 0; j < HC; ++j) {
+    const int r = (j * NW + wave) * RI + lane / KP, p = lane % KP;
+    at_k[j] = r * (2 * HD) + k_piece<HD>(r, p) * 16;
+    at_v[j] = r * (2 * HD) + v_piece<HD>(r, p) * 16;
+  }
+  auto copy16 = [](const uint8_t* base, uint4* dst, int lane_off, int off) __attribute__((always_inline)) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0xffffffffu, 0x00020000), (lds_void*)dst, 16, lane_off, off, 0, 0);
+  };
+  auto copy = [&](uint4* buf, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const Half H = half_at(kb, u);
+#pragma unroll
+      for (int j = 0; j < HC; ++j) {
+        uint4* dst = buf + u * 16 * KP + (j * NW + wave) * 64;
+        copy16(H.k, dst, at_k[j], H.row * (2 * HD));
+        copy16(H.v, dst + TP, at_v[j], H.row * (2 * HD));
+      }
+    }
+  };
+  // 4 bits: a thread takes 32 dims of a row (16 bytes of codes and their
+  // scale) into registers one tile ahead and writes them to LDS as f16
+  constexpr int ST = 2 * kPT * (HD / 32) / (64 * NW);  // blocks of a thread: K's first, then V's
+  uint4 codes[ST];
+  uint32_t scales[ST];
+  auto fetch = [&](int kb) __attribute__((always_inline)) {
+    const Half H0 = half_at(kb, 0), H1 = half_at(kb, 1);
+#pragma unroll
+    for (int j = 0; j < ST; ++j) {
+      const int n = j * 64 * NW + threadIdx.x, r = n / (HD / 32) % kPT, b = n % (HD / 32);
+      const bool isv = n >= kPT * (HD / 32);
+      const uint8_t* base = r < 16 ? (isv ? H0.v : H0.k) : (isv ? H1.v : H1.k);
+      const uint32_t row = (r < 16 ? H0.row : H1.row) + (r & 15);
+      codes[j] = *reinterpret_cast<const uint4*>(base + (row * (HD / 2) + b * 16));
+      scales[j] = *reinterpret_cast<const uint16_t*>(base + ((HD / 2 << P.page_shift) + row * (HD / 16) + b * 2));
+    }
+  };
+  auto unpack = [&](uint4* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < ST; ++j) {
+      const int n = j * 64 * NW + threadIdx.x, r = n / (HD / 32) % kPT, b = n % (HD / 32);
+      const bool isv = n >= kPT * (HD / 32);
+      const h2v d2 = h2_of(scales[j] | scales[j] << 16);
+      const uint32_t w[4] = {codes[j].x, codes[j].y, codes[j].z, codes[j].w};
+      uint4* row = buf + (isv ? TP : 0) + r * KP;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int p = 4 * b + k;
+        row[isv ? v_piece<HD>(r, p) : k_piece<HD>(r, p)] = __builtin_bit_cast(uint4, q4_frag(w[k], d2));
+      }
+    }
+  };
+
+  if (n_tiles > 0) {
+    if constexpr (Q4)
+      fetch(R.base(first));
+    else
+      copy(bufs[0], R.base(first));
+  }
+  // Q^T: dims 32 k + 8 g4 .. + 7
+  h8v q[F][QS];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    bool have;
+    const int64_t q_at = (int64_t)(s.q0 + tok[f]) * A.q_stride + row_of(f, have) * HD;
+#pragma unroll
+    for (int k = 0; k < QS; ++k) {
+      const int64_t a = q_at + k * 32 + g4 * 8;
+      if constexpr (Q16) {
+        q[f][k] = *reinterpret_cast<const h8v*>((const uint16_t*)A.q + a);
+      } else {
+        const float4 x = *reinterpret_cast<const float4*>((const float*)A.q + a);
+        const float4 y = *reinterpret_cast<const float4*>((const float*)A.q + a + 4);
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const _Float16 hi = (_Float16)v[t], lo = (_Float16)(v[t] - (float)hi);
+          q[f][k][t] = c < 8 ? hi : lo;
+        }
+      }
+    }
+  }
+  f4v o[F][DT];
+  float m[F], l[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    m[f] = kNone;
+    l[f] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[f][d] = f4v{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale2 = A.scale * 1.44269504088896341f;
+  // Byte offsets in a tile of this lane's part of K row c, dims 8 g4, and of V
+  // row 4 g4 + c / 4, dims 4 (c % 4); other dims are an xor away.  Kept from the
+  // compiler's view in the loop: the 24 sums would be held in registers.
+  const int vrow = 4 * g4 + (c >> 2);
+  int kx = k_piece<HD>(c, g4) * 16, vx = v_piece<HD>(vrow, (c & 3) >> 1) * 16 + (c & 1) * 8;
+
+  // scores of this wave's columns with the keys of a tile
+  auto scores = [&](const uint4* buf, f4v(&sc)[F][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int f = 0; f < F; ++f) sc[f][0] = sc[f][1] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < QS; ++k)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const h8v ka = *reinterpret_cast<const h8v*>(reinterpret_cast<const char*>(buf + (16 * u + c) * KP) + (kx ^ (64 * k)));
+#pragma unroll
+        for (int f = 0; f < F; ++f) sc[f][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[f][k], sc[f][u], 0, 0, 0);
+      }
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float x = sc[f][j >> 2][j & 3];
+        if constexpr (!Q16) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
+        sc[f][j >> 2][j & 3] = x * scale2;
+      }
+  };
+  auto mask_scores = [&](int kb, uint32_t there, f4v(&sc)[F][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = kb + 16 * (j >> 2) + 4 * g4 + (j & 3);
+        const bool on = (there >> (j >> 2) & 1) && key < cap && key_seen(key, s.p0 + tok[f], A.window, A.sinks);
+        sc[f][j >> 2][j & 3] = on ? sc[f][j >> 2][j & 3] : -__builtin_inff();
+      }
+  };
+  // weights exp2(score - m) as the B operand
+  auto weight = [&](int f, int j, float e, h8v& pf) __attribute__((always_inline)) {
+    const _Float16 hi = (_Float16)e;
+    if constexpr (Q16) {
+      pf[j] = hi;
+    } else {
+      const _Float16 lo = (_Float16)(e - (float)hi);
+      pf[j] = c < 8 ? hi : lo;
+    }
+  };
+  // V^T rows 16 d + c, keys 4 g4 .. + 3 of both halves
+  auto ld_v = [&](const uint4* buf, int d) __attribute__((always_inline)) {
+    u2v x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      x[u] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4*)(
+                                         reinterpret_cast<const char*>(buf + TP + (16 * u + vrow) * KP) + (vx ^ (32 * d)))));
+    return __builtin_bit_cast(h8v, make_uint4(x[0].x, x[0].y, x[1].x, x[1].y));
+  };
+  auto tile = [&](const uint4* buf, int kb, bool whole, uint32_t there) __attribute__((always_inline)) {
+    f4v sc[F][2];
+    scores(buf, sc);
+    if (!whole) mask_scores(kb, there, sc);
+    h8v pf[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      float top = kNone;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[f][j >> 2][j & 3]);
+      top = quad_max4(top);
+      if (__any(top > m[f] + 8.f)) {
+        const float mn = fmaxf(m[f], top), a = exp2_(m[f] - mn);
+        m[f] = mn;
+        l[f] *= a;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[f][d] *= a;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = exp2_(sc[f][j >> 2][j & 3] - m[f]);
+        l[f] += e;
+        weight(f, j, e, pf[f]);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const h8v v = ld_v(buf, d);
+#pragma unroll
+      for (int f = 0; f < F; ++f) o[f][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[f], o[f][d], 0, 0, 0);
+    }
+  };
+
+  // every row of p0 .. p1 sees the whole tile
+  auto all_see = [&](int kb, uint32_t there, int p0, int p1) {
+    return there == 3 && kb + kPT - 1 <= p0 && (A.window == 0 || kb > p1 - A.window || kb + kPT <= A.sinks);
+  };
+  // A row of V that a query does not see must not reach its output even as
+  // 0 x infinity.  In a tile that some query does not see all of, rows that none
+  // of them sees become zeros; true where another one holds a value that is not
+  // finite.  The whole workgroup calls it.
+  auto clean = [&](uint4* buf, int kb, uint32_t there) {
+    bool found = false;
+    for (int j = threadIdx.x; j < TP; j += 64 * NW) {
+      const int r = j / KP, key = kb + r;
+      const bool used = (there >> (r >> 4) & 1) && key < cap && key <= pb &&
+                        (A.window == 0 || key > pa - A.window || key < A.sinks);
+      const uint4 x = buf[TP + j];
+      if (!used)
+        buf[TP + j] = make_uint4(0, 0, 0, 0);
+      else
+        found = found || not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
+    }
+    return __syncthreads_or(found) != 0;
+  };
+  bool odd = false;
+  for (int n = 0; n < n_tiles; ++n) {
+    const int kb = R.base(first + n);
+    uint4* buf = bufs[n & 1];
+    asm volatile("" : "+v"(kx), "+v"(vx));
+    if constexpr (Q4) {
+      unpack(buf);
+      if (n + 1 < n_tiles) fetch(R.base(first + n + 1));
+      lds_sync();
+    } else {
+      // every wave's copies of this tile have landed, and every wave is done
+      // with the buffer that the next ones overwrite
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      lds_sync();
+      if (n + 1 < n_tiles) copy(bufs[(n + 1) & 1], R.base(first + n + 1));
+    }
+    // what the workgroup's rows, and what this wave's, see of it
+    const uint32_t there = (half_at(kb, 0).there ? 1u : 0u) | (half_at(kb, 1).there ? 2u : 0u);
+    if (!all_see(kb, there, pa, pb)) odd = clean(buf, kb, there) || odd;
+    const bool past = kb > wp1, before = A.window > 0 && kb + kPT - 1 <= wp0 - A.window && kb >= A.sinks;
+    if (any && !past && !before) tile(buf, kb, all_see(kb, there, wp0, wp1), there);
+  }
+  if (odd) {
+    // (a broken cache) Row by row and key by key, a wave a row, from memory
+    for (int r = t0 + wave; r < t1; r += NW) {
+      const int t = r / A.gqa, h = g * A.gqa + r % A.gqa, pos = s.p0 + t;
+      constexpr int E = HD / 64;
+      float x[E], y[E], m1 = kNone, l1 = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t qa = (int64_t)(s.q0 + t) * A.q_stride + h * HD + E * lane + e;
+        x[e] = Q16 ? h2f(((const uint16_t*)A.q)[qa]) : ((const float*)A.q)[qa];
+        y[e] = 0.f;
+      }
+      for (int n = 0; n < n_tiles; ++n)
+        for (int key = R.base(first + n), end = key + kPT; key < end; ++key) {
+          const Half H = half_at(key & ~15, 0);
+          if (!H.there || key >= cap || !key_seen(key, pos, A.window, A.sinks)) continue;
+          float sc = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) sc = fmaf(x[e], cache_value<HD, Q4>(H.k, H.row + (key & 15), E * lane + e, P.page_shift), sc);
+          sc = wave_sum(sc) * scale2;
+          const float mn = fmaxf(m1, sc), f = exp2_(m1 - mn), w = exp2_(sc - mn);
+          m1 = mn;
+          l1 = l1 * f + w;
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[e] = y[e] * f + w * cache_value<HD, Q4>(H.v, H.row + (key & 15), E * lane + e, P.page_shift);
+        }
+      const int64_t row = ((int64_t)(at * P.kvh + g) * A.ns + sp) * BM + (r - t0);
+      const float inv = l1 == 0.f ? 0.f : 1.f / l1;
+      if (live > 1 && lane == 0) *reinterpret_cast<float2*>(A.part_ml + row * 2) = make_float2(m1, l1);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (live > 1)
+          A.part[row * HD + E * lane + e] = y[e];
+        else
+          A.out[(int64_t)(s.q0 + t) * A.out_stride + h * HD + E * lane + e] = f2h(y[e] * inv);
+      }
+    }
+    return;
+  }
+
+  // ---- results ----
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const float L = quad_sum4(l[f]);
+    bool have;
+    const int head = row_of(f, have);
+    uint16_t* out = A.out + (int64_t)(s.q0 + tok[f]) * A.out_stride + head * HD + 4 * g4;
+    const bool direct = live <= 1;
+    const float inv = !direct ? 1.f : L == 0.f ? 0.f : 1.f / L;
+    const int64_t row = ((int64_t)(at * P.kvh + g) * A.ns + sp) * BM + (wave * F + f) * RF + (c & (RF - 1));
+    if (!direct && have && lane < RF) *reinterpret_cast<float2*>(A.part_ml + row * 2) = make_float2(m[f], L);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      float x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = o[f][d][r];
+        if constexpr (!Q16) x[r] += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x[r]), 0x128, 0xf, 0xf, true));
+        x[r] *= inv;
+      }
+      if (!have || c >= RF) continue;
+      if (direct)
+        *reinterpret_cast<uint2*>(out + 16 * d) =
+            make_uint2((uint32_t)f2h(x[0]) | (uint32_t)f2h(x[1]) << 16, (uint32_t)f2h(x[2]) | (uint32_t)f2h(x[3]) << 16);
+      else
+        *reinterpret_cast<float4*>(A.part + row * HD + 16 * d + 4 * g4) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+  }
+}
+
+// Merge of the splits: HD / 4 threads a row
+template <int HD, bool Q16>
+__global__ __launch_bounds__(256) void k_attn_chunk_merge(PagedAttnArgs A) {
+  constexpr int BM = kTileRows<HD, Q16>, T = HD / 4, RW = 256 / T;
+  const PagedArgs& P = A.P;
+  const int part = blockIdx.x % (BM / RW), g = blockIdx.x / (BM / RW) % P.kvh, at = blockIdx.x / (BM / RW) / P.kvh;
+  const TileAt ta = find_tile(A, BM, at);
+  const int i = __builtin_amdgcn_readfirstlane(ta.seq), qt = __builtin_amdgcn_readfirstlane(ta.tile);
+  if (i < 0) return;
+  const SeqSpan s = seq_span(P, i);
+  const int rows = s.n * A.gqa, t0 = qt * BM, t1 = min(t0 + BM, rows);
+  const TileRange R = tile_range(s.p0 + t0 / A.gqa, s.p0 + (t1 - 1) / A.gqa, A.window, A.sinks, paged_cap(P));
+  const int per = chunk_per(R.n, A.ns), live = uni((R.n + per - 1) / per);
+  const int r = part * RW + threadIdx.x / T, d = threadIdx.x % T * 4;
+  if (live <= 1 || t0 + r >= t1) return;
+  const int64_t row = (int64_t)(at * P.kvh + g) * A.ns * BM + r;  // + sp * BM
+  float M = kNone, L = 0.f;
+  for (int sp = 0; sp < live; ++sp) M = fmaxf(M, A.part_ml[(row + (int64_t)sp * BM) * 2]);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int sp = 0; sp < live; ++sp) {
+    const int64_t p = row + (int64_t)sp * BM;
+    const float2 st = *reinterpret_cast<const float2*>(A.part_ml + p * 2);
+    const float4 y = *reinterpret_cast<const float4*>(A.part + p * HD + d);
+    const float w = exp2_(st.x - M);
+    L += w * st.y;
+    x.x += w * y.x;
+    x.y += w * y.y;
+    x.z += w * y.z;
+    x.w += w * y.w;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int rr = t0 + r, t = rr / A.gqa, h = g * A.gqa + rr % A.gqa;
+  *reinterpret_cast<uint2*>(A.out + (int64_t)(s.q0 + t) * A.out_stride + h * HD + d) =
+      make_uint2((uint32_t)f2h(x.x * inv) | (uint32_t)f2h(x.y * inv) << 16,
+                 (uint32_t)f2h(x.z * inv) | (uint32_t)f2h(x.w * inv) << 16);
+}
+
+int tile_rows(int hd, bool q16) {
+  return hd == 512 ? (q16 ? kTileRows<512, true> : kTileRows<512, false>)
+                   : (q16 ? kTileRows<256, true> : kTileRows<256, false>);
+}
+// at most this many tiles: each sequence's last may be part full
+int64_t tile_bound(const PagedAttnArgs& a, int bm) {
+  return (int64_t)a.P.n_tok * a.gqa / bm + std::min(a.P.n_seq, a.P.n_tok);
+}
+
+template <int HD, bool Q16>
+int chunk_hd(const PagedAttnArgs& a, bool q4, hipStream_t st) {
+  constexpr int BM = kTileRows<HD, Q16>;
+  const int64_t units = tile_bound(a, BM) * a.P.kvh;
+  if (q4)
+    k_attn_paged_chunk<HD, true, Q16><<<(unsigned)(units * a.ns), 64 * kChunkWaves<HD>, 0, st>>>(a);
+  else
+    k_attn_paged_chunk<HD, false, Q16><<<(unsigned)(units * a.ns), 64 * kChunkWaves<HD>, 0, st>>>(a);
+  E4B_HIP(hipGetLastError());
+  if (a.ns == 1) return E4B_OK;
+  k_attn_chunk_merge<HD, Q16><<<(unsigned)(units * (BM / (1024 / HD))), 256, 0, st>>>(a);
+  E4B_HIP(hipGetLastError());
+  return E4B_OK;
+}
+
+}  // namespace
+
+void plan_attn_paged_chunk(PagedAttnArgs& a, int hd, bool q16) {
+  const int bm = tile_rows(hd, q16);
+  const int64_t units = tile_bound(a, bm) * a.P.kvh;
+  const int64_t seen = a.window ? std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + bm / a.gqa + 1) : a.max_kv;
+  const int64_t tiles = seen / kPT + 2;
+  int64_t ns = std::min<int64_t>((512 + units - 1) / units, tiles / kMinTiles);
+  a.ns = (int)std::max<int64_t>(1, std::min<int64_t>(ns, 64));
+  a.part_floats = a.ns > 1 ? (size_t)units * a.ns * bm * hd : 0;
+  a.ml_floats = a.ns > 1 ? (size_t)units * a.ns * bm * 2 : 0;
+}
+
+int launch_attn_paged_chunk(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st) {
+#define CHUNK(HD) \
+  if (hd == HD) return q16 ? chunk_hd<HD, true>(a, q4, st) : chunk_hd<HD, false>(a, q4, st);
+  CHUNK(128)
+  CHUNK(256)
+  CHUNK(512)
+#undef CHUNK
+  return e4b_fail(E4B_EINVAL, "e4b_k_attn_paged: head_dim %d", hd);
+}

@@ -49,8 +49,8 @@ struct Share {
   int a, b, live;  // live: splits that have any
 };
 DEV Share share_of(const TileRange& R, int ns, int sp, int waves) {
-  const int per = max(waves, (R.n + ns - 1) / ns);
-  return {min(sp * per, R.n), min((sp + 1) * per, R.n), (R.n + per - 1) / per};
+  const int per = max(waves, uni((R.n + ns - 1) / ns));
+  return {min(sp * per, R.n), min((sp + 1) * per, R.n), uni((R.n + per - 1) / per)};
 }
 
 template <int N>
@@ -78,13 +78,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   const PagedArgs& P = A.P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g4 = lane >> 4;
-  const int sp = blockIdx.x % A.ns, unit = blockIdx.x / A.ns;
-  const int rb = unit % A.nrb, g = unit / A.nrb % P.kvh, i = unit / A.nrb / P.kvh;
+  const int unit = uni(blockIdx.x / A.ns), sp = blockIdx.x - unit * A.ns;
+  const int head = uni(unit / A.nrb), rb = unit - head * A.nrb, i = uni(head / P.kvh), g = head - i * P.kvh;
   const SeqSpan s = seq_span(P, i);
+  if ((int64_t)s.n * A.gqa > kPagedFewRows) return;  // k_paged_chunk.hip's
   const int rows = min(min(s.n, A.max_q) * A.gqa - kRows * rb, kRows);
   if (rows <= 0) return;
   const int cap = paged_cap(P);
-  const int r0 = kRows * rb, t_first = r0 / A.gqa, t_last = (r0 + rows - 1) / A.gqa;
+  const int r0 = kRows * rb, t_first = uni(r0 / A.gqa), t_last = uni((r0 + rows - 1) / A.gqa);
   const int p_first = s.p0 + t_first, p_last = s.p0 + t_last;
   const TileRange R = tile_range(p_first, p_last, A.window, A.sinks, cap);
   const Share sh = share_of(R, A.ns, sp, W);
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   // the column's sum over the lane groups, the two columns of a row, the waves
   l = quad_sum4(l);
   lds_sync();  // every wave is done with the queries
-  const int nr = min(A.max_rows, kRows);  // rows that LDS has room for
+  const int nr = min(A.max_q * A.gqa, kRows);  // rows that LDS has room for
   float* ml = lds + W * nr * LD;
 #pragma unroll
   for (int h = 0; h < NH; ++h)
@@ -393,10 +394,11 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs A) {
   __shared__ float red[4];
   __shared__ __align__(16) float sum[NG][HD];
   const PagedArgs& P = A.P;
-  const int nr = min(A.max_rows, kRows);
+  const int nr = min(A.max_q * A.gqa, kRows);
   const int r = blockIdx.x % nr, unit = blockIdx.x / nr;
   const int rb = unit % A.nrb, g = unit / A.nrb % P.kvh, i = unit / A.nrb / P.kvh;
   const SeqSpan s = seq_span(P, i);
+  if ((int64_t)s.n * A.gqa > kPagedFewRows) return;
   const int rows = min(min(s.n, A.max_q) * A.gqa - kRows * rb, kRows);
   if (r >= rows) return;
   const int r0 = kRows * rb;
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs A) {
 template <int HD>
 int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
   constexpr int W = kStreams<HD>;
-  const int nr = std::min(a.max_rows, kRows), units = a.P.n_seq * a.P.kvh * a.nrb;
+  const int nr = std::min(a.max_q * a.gqa, kRows), units = a.P.n_seq * a.P.kvh * a.nrb;
   const size_t lds = std::max((size_t)W * nr * (HD + 4) * 4 + W * kRows * 8, (size_t)HD * 32);
   const dim3 grid((unsigned)(units * a.ns));
   auto go = [&](auto* kernel) {
@@ -466,14 +468,14 @@ int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
 
 void plan_attn_paged_few(PagedAttnArgs& a, int hd) {
   const int W = hd == 512 ? kStreams<512> : kStreams<256>;
-  a.nrb = (a.max_rows + kRows - 1) / kRows;
+  a.nrb = (a.max_q * a.gqa + kRows - 1) / kRows;
   const int64_t units = (int64_t)a.P.n_seq * a.P.kvh * a.nrb;
   const int64_t seen = a.window ? std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + a.max_q) : a.max_kv;
   const int64_t tiles = seen / kPT + 2;
   int64_t ns = std::min<int64_t>((512 + units - 1) / units, tiles / W);
   if (tiles <= 2 * W) ns = 1;
   a.ns = (int)std::max<int64_t>(1, std::min<int64_t>(ns, kPagedMaxSplits));
-  const int nr = std::min(a.max_rows, kRows);
+  const int nr = std::min(a.max_q * a.gqa, kRows);
   a.part_floats = a.ns > 1 ? (size_t)units * a.ns * nr * hd : 0;
   a.ml_floats = a.ns > 1 ? (size_t)units * a.ns * nr * 2 : 0;
 }

@@ -111,9 +111,10 @@ struct PagedAttnArgs {
   int qh, gqa, window, sinks;
   float scale;
   int max_q, max_kv;        // bounds of a sequence's tokens (<= n_tok) and positions
-  // the plan: rows (tokens x heads of a group) that a sequence has at most,
-  // blocks of them, splits of the keys, and where the splits' results go
-  int max_rows, nrb, ns;
+  // the plan: blocks of rows (tokens x heads of a group) of a sequence, splits
+  // of the keys, and where the splits' results go
+  int nrb, ns;
+  int few_rows;             // chunks: sequences with no more rows than this are left out
   size_t part_floats, ml_floats;
   float* part;
   float* part_ml;
@@ -121,6 +122,8 @@ struct PagedAttnArgs {
 // a few query rows per sequence and KV head (k_paged_decode.hip)
 void plan_attn_paged_few(PagedAttnArgs& a, int hd);
 int launch_attn_paged_few(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
-constexpr int kPagedFewRows = 16;  // most rows of a sequence and KV head that k_paged_decode.hip takes
-int launch_attn_paged(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
+constexpr int kPagedFewRows = 16;  // most rows of a sequence and KV head that it takes
+// any number (k_paged_chunk.hip)
+void plan_attn_paged_chunk(PagedAttnArgs& a, int hd, bool q16);
+int launch_attn_paged_chunk(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
 #endif

@@ -130,32 +130,58 @@ extern "C" int e4b_k_kv_gather(const e4b_paged_kv* kv, const e4b_kv_batch* batch
                           (hipStream_t)stream);
 }
 
-// splits' outputs, then their maxima and sums
-static size_t scratch_bytes(const PagedAttnArgs& a) {
-  return E4B_ALIGN256(a.part_floats * sizeof(float)) + a.ml_floats * sizeof(float);
+// An attention call: the sequences with few query rows go to one kernel, the
+// others to another.
+struct AttnPlan {
+  PagedAttnArgs few, chunk;
+  bool use_few = false, use_chunk = false;
+};
+static size_t scratch_bytes(const PagedAttnArgs& a) {  // splits' outputs, then their maxima and sums
+  return E4B_ALIGN256(a.part_floats * sizeof(float)) + E4B_ALIGN256(a.ml_floats * sizeof(float));
+}
+static size_t scratch_bytes(const AttnPlan& p) {
+  return (p.use_few ? scratch_bytes(p.few) : 0) + (p.use_chunk ? scratch_bytes(p.chunk) : 0);
+}
+static uint8_t* give_scratch(PagedAttnArgs& a, uint8_t* ws) {
+  a.part = (float*)ws;
+  a.part_ml = (float*)(ws + E4B_ALIGN256(a.part_floats * sizeof(float)));
+  return ws + scratch_bytes(a);
 }
 
-// the checks of an attention call; *a is complete but for its pointers
+// the checks of an attention call; *plan is complete but for pointers and scale
 static int attn_setup(const char* fn, const e4b_paged_kv* kv, const e4b_kv_batch* batch, int q_dtype, int q_heads,
-                      int window, int sinks, PagedAttnArgs* a, bool* empty) {
-  int rc = check_call(fn, kv, batch, &a->P, empty);
+                      int window, int sinks, AttnPlan* plan, bool* empty) {
+  PagedAttnArgs a{};
+  int rc = check_call(fn, kv, batch, &a.P, empty);
   if (rc) return rc;
   if (q_heads < 1 || q_heads > 4096 || q_heads % kv->kv_heads)
     return e4b_fail(E4B_EINVAL, "%s: %d query heads over %d KV heads", fn, q_heads, kv->kv_heads);
   if (q_dtype != E4B_DT_F32 && q_dtype != E4B_DT_F16)
     return e4b_fail(E4B_EINVAL, "%s: q dtype %d (E4B_DT_F32 or E4B_DT_F16)", fn, q_dtype);
   if (window < 0 || sinks < 0) return e4b_fail(E4B_EINVAL, "%s: window %d, sinks %d", fn, window, sinks);
-  a->qh = q_heads;
-  a->gqa = q_heads / kv->kv_heads;
-  a->window = window;
-  a->sinks = window ? sinks : 0;
-  a->ns = 1;
-  a->part_floats = a->ml_floats = 0;
   if (*empty) return E4B_OK;
-  a->max_q = std::min(batch->max_q, batch->n_tok);
-  a->max_kv = batch->max_kv;
-  a->max_rows = (int)std::min<int64_t>((int64_t)a->max_q * a->gqa, 1 << 30);
-  if (a->max_rows <= kPagedFewRows) plan_attn_paged_few(*a, kv->head_dim);
+  if ((int64_t)batch->n_tok * q_heads > (1 << 30))
+    return e4b_fail(E4B_EINVAL, "%s: %d tokens of %d heads are more than 2^30 rows", fn, batch->n_tok, q_heads);
+  a.qh = q_heads;
+  a.gqa = q_heads / kv->kv_heads;
+  a.window = window;
+  a.sinks = window ? sinks : 0;
+  a.max_q = std::min(batch->max_q, batch->n_tok);
+  a.max_kv = batch->max_kv;
+  plan->use_chunk = a.max_q * a.gqa > kPagedFewRows;
+  // Short sequences beside long ones: where all are as long as the longest
+  // there are none, and a launch is saved
+  plan->use_few = !plan->use_chunk || (a.gqa <= kPagedFewRows && (int64_t)batch->n_seq * a.max_q > batch->n_tok);
+  if (plan->use_few) {
+    plan->few = a;
+    plan->few.max_q = std::min(a.max_q, kPagedFewRows / a.gqa);
+    plan_attn_paged_few(plan->few, kv->head_dim);
+  }
+  if (plan->use_chunk) {
+    plan->chunk = a;
+    plan->chunk.few_rows = plan->use_few ? kPagedFewRows : 0;
+    plan_attn_paged_chunk(plan->chunk, kv->head_dim, q_dtype == E4B_DT_F16);
+  }
   return E4B_OK;
 }
 
@@ -163,11 +189,11 @@ extern "C" int e4b_attn_paged_ws_bytes(const e4b_paged_kv* kv, const e4b_kv_batc
                                        int window, int sinks, size_t* bytes) {
   const char* fn = "e4b_attn_paged_ws_bytes";
   if (!bytes) return e4b_fail(E4B_EINVAL, "%s: null result", fn);
-  PagedAttnArgs a;
+  AttnPlan plan;
   bool empty;
-  int rc = attn_setup(fn, kv, batch, q_dtype, q_heads, window, sinks, &a, &empty);
+  int rc = attn_setup(fn, kv, batch, q_dtype, q_heads, window, sinks, &plan, &empty);
   if (rc) return rc;
-  *bytes = scratch_bytes(a);
+  *bytes = scratch_bytes(plan);
   return E4B_OK;
 }
 
@@ -175,15 +201,15 @@ extern "C" int e4b_k_attn_paged(const e4b_paged_kv* kv, const e4b_kv_batch* batc
                                 int64_t q_stride, int q_heads, float scale, int window, int sinks, void* out_f16,
                                 int64_t out_stride, void* ws, size_t ws_bytes, void* stream) {
   const char* fn = "e4b_k_attn_paged";
-  PagedAttnArgs a;
+  AttnPlan plan;
   bool empty;
-  int rc = attn_setup(fn, kv, batch, q_dtype, q_heads, window, sinks, &a, &empty);
+  int rc = attn_setup(fn, kv, batch, q_dtype, q_heads, window, sinks, &plan, &empty);
   if (rc) return rc;
   if (!(scale - scale == 0.f)) return e4b_fail(E4B_EINVAL, "%s: scale is not finite", fn);
   if (empty) return E4B_OK;
   if ((rc = check_rows(fn, "q", q, q_dtype, q_stride, q_heads, kv->head_dim))) return rc;
   if ((rc = check_rows(fn, "out", out_f16, E4B_DT_F16, out_stride, q_heads, kv->head_dim))) return rc;
-  if (const size_t need = scratch_bytes(a)) {
+  if (const size_t need = scratch_bytes(plan)) {
     if (ws && (ws_bytes < need || !aligned(ws, 16)))
       return e4b_fail(E4B_EINVAL, "%s: %zu bytes of scratch where %zu, 16-byte aligned, are needed", fn, ws_bytes, need);
     if (!ws) {
@@ -191,13 +217,20 @@ extern "C" int e4b_k_attn_paged(const e4b_paged_kv* kv, const e4b_kv_batch* batc
       if ((rc = e4b_workspace(need, &w, (hipStream_t)stream))) return rc;
       ws = w.buf;
     }
-    a.part = (float*)ws;
-    a.part_ml = (float*)((uint8_t*)ws + E4B_ALIGN256(a.part_floats * sizeof(float)));
   }
-  a.q = q;
-  a.q_stride = q_stride;
-  a.out = (uint16_t*)out_f16;
-  a.out_stride = out_stride;
-  a.scale = scale;
-  return launch_attn_paged(a, kv->head_dim, kv->type == E4B_KV_Q4, q_dtype == E4B_DT_F16, (hipStream_t)stream);
+  uint8_t* at = (uint8_t*)ws;
+  const bool q4 = kv->type == E4B_KV_Q4, q16 = q_dtype == E4B_DT_F16;
+  for (PagedAttnArgs* a : {plan.use_chunk ? &plan.chunk : nullptr, plan.use_few ? &plan.few : nullptr}) {
+    if (!a) continue;
+    a->q = q;
+    a->q_stride = q_stride;
+    a->out = (uint16_t*)out_f16;
+    a->out_stride = out_stride;
+    a->scale = scale;
+    at = give_scratch(*a, at);
+    rc = a == &plan.chunk ? launch_attn_paged_chunk(*a, kv->head_dim, q4, q16, (hipStream_t)stream)
+                          : launch_attn_paged_few(*a, kv->head_dim, q4, q16, (hipStream_t)stream);
+    if (rc) return rc;
+  }
+  return E4B_OK;
 }

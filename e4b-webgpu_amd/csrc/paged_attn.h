@@ -10,6 +10,10 @@ typedef float f4v __attribute__((ext_vector_type(4)));
 
 constexpr int kPT = 32;  // keys per tile: two 16-key halves, each inside one page
 
+// a value that is the same in all lanes, in a scalar register (an integer
+// division leaves it in a vector one, and what depends on it with it)
+DEV int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Tiles of the keys that queries at positions p0 .. p1 see, in the order of
 // the keys: `sink` tiles from 0 on, then the ones from `from` on.
 struct TileRange {
