@@ -86,21 +86,16 @@ DEV void head_rms(T (&x)[E], const float* w, float eps) {
 }
 
 // Pairs (d, d + hd / 2), d < angles: lane l < 32 holds dims E l .. and lane
-// l + 32 their partners.  The angle pos * inv_freq[d] is made and reduced in
-// 64 bits: at position 30000 a 32-bit product is off by up to 2^-10 of a
-// radian, several roundings of an f16 result.
-template <int E, typename T>
-DEV void rotate(T (&x)[E], const float* inv_freq, int angles, int pos) {
+// l + 32 their partners.  turns: (cos, sin) of the token's pairs.
+template <int E, typename T, typename T2>
+DEV void rotate(T (&x)[E], const T2* turns, int angles) {
   const int lane = threadIdx.x & 63, d0 = E * (lane & 31);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const T other = __shfl_xor(x[i], 32, 64);
     if (d0 + i < angles) {
-      const double a = (double)pos * (double)inv_freq[d0 + i];
-      const double turn = 6.283185307179586476925;
-      T s, c;
-      sin_cos(fma(-rint(a * (1.0 / turn)), turn, a), s, c);
-      x[i] = lane < 32 ? x[i] * c - other * s : x[i] * c + other * s;
+      const T2 t = turns[d0 + i];
+      x[i] = lane < 32 ? x[i] * (T)t.x - other * (T)t.y : x[i] * (T)t.x + other * (T)t.y;
     }
   }
 }
@@ -159,35 +154,27 @@ DEV void st_q4(uint8_t* codes, uint8_t* scales, const double (&x)[E]) {
 
 // Append: workgroup (token, part of the heads), a wave takes every
 // (4 gridDim.y)-th head row of [q heads | k heads | v heads], E = HD / 64 dims
-// a lane.  K and V of a 4-bit cache are prepared in 64 bits (st_q4), all else
-// in 32.  What bounds it: latency (a load of the row, the sequence's entries
-// and the table's, the store); bytes once there are thousands of tokens.
+// a lane, the next row requested before one is worked on.  K and V of a 4-bit
+// cache are prepared in 64 bits (st_q4), all else in 32.
+// The angle pos * inv_freq[d] is made and reduced in 64 bits: at position
+// 30000 a 32-bit product is off by up to 2^-10 of a radian, several roundings
+// of an f16 result.  Its sine and cosine are taken once a token, one pair a
+// thread (every head's wave for itself: 57 us for 2600 tokens of 32 heads).
+// What bounds it: latency (a load of the row, the sequence's entries and the
+// table's, the store); bytes once there are thousands of tokens.
 template <int HD, bool Q4, bool X16>
 __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs A) {
   constexpr int E = HD / 64;
   using T = std::conditional_t<Q4, double, float>;
+  using T2 = std::conditional_t<Q4, double2, float2>;
+  __shared__ T2 turns[HD / 2];
   const PagedArgs& P = A.P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x;
-  const int i = __builtin_amdgcn_readfirstlane(seq_of_token(P, t));
-  if (i >= P.n_seq) return;  // behind the last sequence
-  const SeqSpan s = seq_span(P, i);
-  const int pos = s.p0 + (t - s.q0);
-  if (pos < 0 || t < s.q0 || t - s.q0 >= s.n) return;
-  const int pg = paged_page(table_row(P, i), P.table_stride, P.page_shift, P.n_pages, pos);
-  const int row = pos & ((1 << P.page_shift) - 1);
+  const int t = blockIdx.x, step = 4 * gridDim.y;
   const int heads = A.qh + (A.v_is_k ? 1 : 2) * P.kvh;
-  auto put = [&](uint8_t* pool, int g, const T(&x)[E]) {
-    if (pg < 0) return;
-    uint8_t* b = pool + paged_block<Q4, HD>(P, pg, g);
-    if constexpr (Q4)
-      st_q4<E>(b + row * (HD / 2), b + (HD / 2 << P.page_shift) + row * (HD / 16), x);
-    else
-      st_f16<E>(b + (row * HD + E * lane) * 2, x);
-  };
-  for (int h = blockIdx.y * 4 + wave; h < heads; h += 4 * gridDim.y) {
-    if (h < A.qh && !A.q) continue;
-    float x[E];
+  int h = blockIdx.y * 4 + wave;
+  if (!A.q && h < A.qh) h += (A.qh - h + step - 1) / step * step;  // the first row that is wanted
+  auto load = [&](int h, float(&x)[E]) __attribute__((always_inline)) {
     const int64_t at = (int64_t)t * A.x_stride + h * HD + E * lane;
     if constexpr (X16) {
       uint32_t w[E / 2];
@@ -197,9 +184,38 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs A) {
     } else {
       ld_f32<E>((const float*)A.x + at, x);
     }
+  };
+  float x[E], ahead[E];
+  if (h < heads) load(h, ahead);
+  const int i = __builtin_amdgcn_readfirstlane(seq_of_token(P, t));
+  if (i >= P.n_seq) return;  // behind the last sequence
+  const SeqSpan s = seq_span(P, i);
+  const int pos = s.p0 + (t - s.q0);
+  if (pos < 0 || t < s.q0 || t - s.q0 >= s.n) return;
+  if ((int)threadIdx.x < A.angles) {
+    const double a = (double)pos * (double)A.inv_freq[threadIdx.x], turn = 6.283185307179586476925;
+    T sn, cs;
+    sin_cos(fma(-rint(a * (1.0 / turn)), turn, a), sn, cs);
+    turns[threadIdx.x] = T2{cs, sn};
+  }
+  lds_sync();
+  const int pg = paged_page(table_row(P, i), P.table_stride, P.page_shift, P.n_pages, pos);
+  const int row = pos & ((1 << P.page_shift) - 1);
+  auto put = [&](uint8_t* pool, int g, const T(&x)[E]) {
+    if (pg < 0) return;
+    uint8_t* b = pool + paged_block<Q4, HD>(P, pg, g);
+    if constexpr (Q4)
+      st_q4<E>(b + row * (HD / 2), b + (HD / 2 << P.page_shift) + row * (HD / 16), x);
+    else
+      st_f16<E>(b + (row * HD + E * lane) * 2, x);
+  };
+  for (; h < heads; h += step) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = ahead[j];
+    if (h + step < heads) load(h + step, ahead);
     if (h < A.qh) {
       if (A.qw) head_rms<E>(x, A.qw, A.eps);
-      rotate<E>(x, A.inv_freq, A.angles, pos);
+      rotate<E>(x, turns, A.angles);
       const int64_t o = (int64_t)t * A.q_stride + h * HD + E * lane;
       if (A.q16) {
         st_f16<E>((uint16_t*)A.q + o, x);
@@ -214,14 +230,14 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs A) {
       }
       continue;
     }
-    const int g = (h - A.qh) % P.kvh;
+    const int g = h < A.qh + P.kvh ? h - A.qh : h - A.qh - P.kvh;
     const bool isk = h < A.qh + P.kvh;
     T y[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) y[j] = (T)x[j];
     if (isk) {
       if (A.kw) head_rms<E>(y, A.kw, A.eps);
-      rotate<E>(y, A.inv_freq, A.angles, pos);
+      rotate<E>(y, turns, A.angles);
       put(P.k, g, y);
       if (!A.v_is_k) continue;
 #pragma unroll

@@ -31,10 +31,11 @@ namespace {
 
 constexpr int kRows = 8;
 constexpr int kWaves = 8;
-// waves that share a tile, each with 256 of V's dims at most (a wave's output
-// is HD / 4 registers else); both compute the scores
+// Waves that share a tile.  Head dim 512 has no room for all of the output
+// (128 registers) beside the rows in flight: two waves take half of the dims
+// each, add up their halves of the scores through LDS, and keep half of V's.
 template <int HD>
-constexpr int kParts = HD == 512 ? 2 : 1;
+constexpr int kParts = HD / 256 > 1 ? 2 : 1;
 template <int HD>
 constexpr int kStreams = kWaves / kParts<HD>;  // tiles at a time in a workgroup
 
@@ -44,14 +45,26 @@ struct RowOf {
 };
 DEV RowOf row_of(const PagedAttnArgs& A, int g, int r) { return {r / A.gqa, g * A.gqa + r % A.gqa}; }
 
+// Splits.  A workgroup fills a CU, so there are at most as many as CUs (one
+// token at 32767 positions in 4 bits 15.7 us with 256 workgroups, 21.2 with
+// 512).  A split is a launch more (about 4 us), and what it saves is the time
+// in which one CU takes in its share: none up to 7 tiles (one token at 128
+// positions 7.2 us in one workgroup, 9.0 in two), shares of 4 tiles above (at
+// 300 positions 10.6 us, 12.9 in one workgroup; shares of 2 10.7 us).
+constexpr int kMinShare = 4, kUnsplit = 7, kMaxGroups = 256;
+
 // the share of split sp: tiles a .. b - 1
 struct Share {
   int a, b, live;  // live: splits that have any
 };
-DEV Share share_of(const TileRange& R, int ns, int sp, int waves) {
-  const int per = max(waves, uni((R.n + ns - 1) / ns));
+DEV Share share_of(const TileRange& R, int ns, int sp) {
+  const int per = max(kMinShare, uni((R.n + ns - 1) / ns));
   return {min(sp * per, R.n), min((sp + 1) * per, R.n), uni((R.n + per - 1) / per)};
 }
+
+// what a page that is not there is read as (never written): codes of a page
+// and 16 rows' scales, or 16 rows, whichever is more
+__device__ uint4 zeros[(512 / 2 * 256 + 16 * 32) / 16];
 
 template <int N>
 DEV void ld_dwords(const uint8_t* p, uint32_t* x) {
@@ -72,7 +85,7 @@ DEV void ld_dwords(const uint8_t* p, uint32_t* x) {
 
 template <int HD, bool Q4, bool Q16>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs A) {
-  constexpr int W = kStreams<HD>, VP = kParts<HD>, NH = HD / 128 / VP, QS = HD / 32;
+  constexpr int W = kStreams<HD>, VP = kParts<HD>, HW = HD / VP, NH = HW / 128, QS = HW / 32;  // HW: dims of a wave
   constexpr int LD = HD + 4;  // floats between rows in LDS
   extern __shared__ __align__(16) float lds[];  // queries; later [W][rows][LD] outputs, [W][8][2] maxima and sums
   const PagedArgs& P = A.P;
@@ -88,38 +101,124 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   const int r0 = kRows * rb, t_first = uni(r0 / A.gqa), t_last = uni((r0 + rows - 1) / A.gqa);
   const int p_first = s.p0 + t_first, p_last = s.p0 + t_last;
   const TileRange R = tile_range(p_first, p_last, A.window, A.sinks, cap);
-  const Share sh = share_of(R, A.ns, sp, W);
+  const Share sh = share_of(R, A.ns, sp);
   if (sh.a >= sh.b && !(sp == 0 && R.n == 0)) return;
   const RowOf ro = row_of(A, g, r0 + min(c & 7, rows - 1));
   const int pos = s.p0 + ro.tok;  // of this lane's column
   const table_ptr trow = table_row(P, i);
 
-  // Q^T fragments, dims in the order that K's rows are read, through LDS: in
-  // registers they would cost every wave HD / 8 of them
-  h8v* qf = reinterpret_cast<h8v*>(lds);
-  {
-    const int64_t at = (int64_t)(s.q0 + ro.tok) * A.q_stride + ro.head * HD;
+
+  // This stream's tiles: first those that every row sees all of, then the
+  // others (a loop with both kinds kept two copies of the output registers)
+  const int stream = wave / VP, part = wave % VP;  // part: the wave's dims are HW part ..
+  const int wa = R.sink - R.from + (A.window > 0 ? max(0, p_last - A.window + kPT) / kPT : 0);
+  const int wb = R.sink - R.from + max(0, min(p_first, cap - 1) + 1) / kPT;
+  const int a0 = min(max(sh.a, wa), sh.b), n_whole = max(0, min(sh.b, wb) - a0), n_all = sh.b - sh.a;
+  auto base_of = [&](int v) {
+    const int before = a0 - sh.a, e = v - n_whole;
+    return R.base(v < n_whole ? a0 + v : e < before ? sh.a + e : v + sh.a);
+  };
+  // A tile's halves: their pages' blocks and the first rows there.  A half
+  // without a page is read from zeros.
+  struct Where {
+    const uint8_t *k[2], *v[2];
+    int row[2], kb;
+    uint32_t there;
+  };
+  auto locate = [&](int kb) __attribute__((always_inline)) {
+    Where w;
+    w.kb = kb;
+    w.there = 0;
 #pragma unroll
-    for (int k0 = 0; k0 < QS; k0 += kWaves) {
-      const int k = k0 + wave;
-      if (k < QS) {
-        const int d = Q4 ? (g4 * QS + k) * 8 : k * 32 + g4 * 8;
-        h8v q;
-        if constexpr (Q16) {
-          q = *reinterpret_cast<const h8v*>((const uint16_t*)A.q + at + d);
-        } else {
-          const float4 a = *reinterpret_cast<const float4*>((const float*)A.q + at + d);
-          const float4 b = *reinterpret_cast<const float4*>((const float*)A.q + at + d + 4);
-          const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    for (int u = 0; u < 2; ++u) {
+      const int p = kb + 16 * u, b = p >> P.page_shift;
+      const uint32_t pg = trow[min(b, P.table_stride - 1)];
+      const bool is = b < P.table_stride && pg < (uint32_t)P.n_pages;
+      const int64_t blk = paged_block<Q4, HD>(P, is ? (int)pg : 0, g);
+      w.k[u] = is ? P.k + blk : (const uint8_t*)zeros;
+      w.v[u] = is ? P.v + blk : (const uint8_t*)zeros;
+      w.row[u] = is ? p & ((1 << P.page_shift) - 1) : 0;
+      w.there |= is ? 1u << u : 0u;
+    }
+    return w;
+  };
+  // K: row 16 u + c; kd: the scales of this lane's blocks, two a dword
+  uint32_t kw[2][Q4 ? QS : 4 * QS], kd[2];
+  auto load_k = [&](const Where& w, int u) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      const uint32_t at = (w.row[u] + c) * (HD / 2) + part * (HW / 2) + g4 * (HW / 8);
 #pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            const _Float16 hi = (_Float16)v[t], lo = (_Float16)(v[t] - (float)hi);
-            q[t] = c < 8 ? hi : lo;
-          }
-        }
-        qf[k * 64 + lane] = q;
+      for (int k = 0; k < QS; k += 4) ld_dwords<4>(w.k[u] + (at + k * 4), kw[u] + k);
+      const uint8_t* ks = w.k[u] + (uint32_t)((HD / 2 << P.page_shift) + (w.row[u] + c) * (HD / 16) + part * (HW / 16) + g4 * (HW / 64));
+      if constexpr (HW == 128)
+        kd[u] = *reinterpret_cast<const uint16_t*>(ks);
+      else
+        kd[u] = *reinterpret_cast<const uint32_t*>(ks);
+    } else {
+      const uint32_t at = ((w.row[u] + c) * HD + part * HW + g4 * 8) * 2;
+#pragma unroll
+      for (int k = 0; k < QS; ++k) ld_dwords<4>(w.k[u] + (at + k * 64), kw[u] + 4 * k);
+    }
+  };
+  // V: this lane's 8 keys 16 u + 4 g4 + r, some dims of each, and their scales
+  uint32_t v[8][Q4 ? NH : 4 * NH];
+  uint16_t vd[8];
+  auto load_v = [&](const Where& w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int u = k >> 2, row = w.row[u] + 4 * g4 + (k & 3);
+      if constexpr (Q4) {
+        ld_dwords<NH>(w.v[u] + (uint32_t)(row * (HD / 2) + part * (HW / 2) + c * 4 * NH), v[k]);
+        vd[k] = *reinterpret_cast<const uint16_t*>(
+            w.v[u] + (uint32_t)((HD / 2 << P.page_shift) + row * (HD / 16) + part * (HW / 16) + (c * NH / 4) * 2));
+      } else {
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+          ld_dwords<4>(w.v[u] + (uint32_t)((row * HD + part * HW + c * 8 + h * 128) * 2), v[k] + 4 * h);
       }
     }
+  };
+  constexpr bool kBoth = Q4 || HW <= 128;  // registers for both halves of K of the next tile beside V and the output
+
+  // Q^T fragments, dims in the order that K's rows are read, through LDS: in
+  // registers they would cost every wave HD / 8 of them.  Their loads go out
+  // first, then the first tile's.
+  h8v* qf = reinterpret_cast<h8v*>(lds);
+  constexpr int QF = HD / 32, QN = (QF + kWaves - 1) / kWaves;  // fragments, and of a wave
+  uint32_t qraw[QN][Q16 ? 4 : 8];
+  const int64_t q_at = (int64_t)(s.q0 + ro.tok) * A.q_stride + ro.head * HD;
+#pragma unroll
+  for (int j = 0; j < QN; ++j) {
+    const int f = min(j * kWaves + wave, QF - 1), k = f % QS, d = f / QS * HW + (Q4 ? (g4 * QS + k) * 8 : k * 32 + g4 * 8);
+    const uint8_t* p = (const uint8_t*)A.q + (q_at + d) * (Q16 ? 2 : 4);
+    ld_dwords<4>(p, qraw[j]);
+    if constexpr (!Q16) ld_dwords<4>(p + 16, qraw[j] + 4);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  int at = stream;  // of this stream's tiles
+  Where next{};
+  if (at < n_all) {
+    next = locate(base_of(at));
+    load_k(next, 0);
+    if constexpr (kBoth) load_k(next, 1);
+    load_v(next);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < QN; ++j) {
+    const int k = j * kWaves + wave;
+    h8v q;
+    if constexpr (Q16) {
+      q = __builtin_bit_cast(h8v, make_uint4(qraw[j][0], qraw[j][1], qraw[j][2], qraw[j][3]));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const float x = __uint_as_float(qraw[j][t]);
+        const _Float16 hi = (_Float16)x, lo = (_Float16)(x - (float)hi);
+        q[t] = c < 8 ? hi : lo;
+      }
+    }
+    if (k < QF) qf[k * 64 + lane] = q;
   }
   lds_sync();
   f4v o[NH][8];
@@ -129,96 +228,59 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
     for (int t = 0; t < 8; ++t) o[h][t] = f4v{0.f, 0.f, 0.f, 0.f};
   float m = kNone, l = 0.f;  // of this lane's column; l over this lane's keys alone
   const float scale2 = A.scale * 1.44269504088896341f;
-
-  const int stream = wave / VP, part = wave % VP;  // part: V's dims 256 part .. of head dim 512
   int qat = lane;
-  auto tile = [&](int kb, auto whole_tag) __attribute__((always_inline)) {
+  [[maybe_unused]] int round = 0;
+
+  auto tile = [&](auto whole_tag) __attribute__((always_inline)) {
     constexpr bool whole = decltype(whole_tag)::value;
     asm volatile("" : "+v"(qat));  // the query fragments stay in LDS
-    // where the two halves lie
-    const uint8_t *kh[2], *vh[2];
-    [[maybe_unused]] bool there[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int pg = paged_page(trow, P.table_stride, P.page_shift, P.n_pages, kb + 16 * u);
-      there[u] = pg >= 0;
-      const int64_t blk = paged_block<Q4, HD>(P, max(pg, 0), g);
-      kh[u] = P.k + blk;
-      vh[u] = P.v + blk;
-    }
-    const int r16 = kb & ((1 << P.page_shift) - 1) & ~15;
-    const int row0[2] = {r16, (r16 + 16) & ((1 << P.page_shift) - 1)};
+    const Where cur = next;
+    const int kb = cur.kb;
+    const bool more = at + W < n_all;
+    if (more) next = locate(base_of(at + W));
     // keys that this lane weighs: bit 4 u + r is key kb + 16 u + 4 g4 + r
-    uint32_t seen = 0xff;
+    uint32_t seen = (cur.there & 1 ? 0xfu : 0u) | (cur.there & 2 ? 0xf0u : 0u);
     if constexpr (!whole) {
-      seen = 0;
+      uint32_t by = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = kb + 16 * u + 4 * g4 + r;
-          if (there[u] && key < cap && key_seen(key, pos, A.window, A.sinks)) seen |= 1u << (4 * u + r);
-        }
-    }
-    // K: row 16 u + c
-    uint32_t kw[2][Q4 ? QS : 4 * QS], kd[2][HD == 128 ? 1 : HD / 256];  // kd: scales of this lane's blocks, two a dword
-    auto load_k = [&](int u) __attribute__((always_inline)) {
-      if constexpr (Q4) {
-        const uint32_t at = (row0[u] + c) * (HD / 2) + g4 * (HD / 8);
-#pragma unroll
-        for (int k = 0; k < QS; k += 4) ld_dwords<4>(kh[u] + (at + k * 4), kw[u] + k);
-        const uint8_t* ks = kh[u] + (uint32_t)((HD / 2 << P.page_shift) + (row0[u] + c) * (HD / 16) + g4 * (HD / 64));
-        if constexpr (HD == 128)
-          kd[u][0] = *reinterpret_cast<const uint16_t*>(ks);
-        else
-          ld_dwords<HD / 256>(ks, kd[u]);
-      } else {
-        const uint32_t at = ((row0[u] + c) * HD + g4 * 8) * 2;
-#pragma unroll
-        for (int k = 0; k < QS; ++k) ld_dwords<4>(kh[u] + (at + k * 64), kw[u] + 4 * k);
+      for (int k = 0; k < 8; ++k) {
+        const int key = kb + 16 * (k >> 2) + 4 * g4 + (k & 3);
+        if (key < cap && key_seen(key, pos, A.window, A.sinks)) by |= 1u << k;
       }
-    };
+      seen &= by;
+    }
     f4v sc[2] = {f4v{0.f, 0.f, 0.f, 0.f}, f4v{0.f, 0.f, 0.f, 0.f}};
     auto scores = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < QS; ++k) {
         h8v a;
         if constexpr (Q4) {
-          const uint32_t x = kd[u][k / 8];
-          a = q4_frag(kw[u][k], h2_of((k / 4) & 1 ? hi_halves(x, x) : lo_halves(x, x)));
+          const uint32_t x = kd[u];
+          a = q4_frag(kw[u][k], h2_of(k / 4 ? hi_halves(x, x) : lo_halves(x, x)));
         } else {
           a = __builtin_bit_cast(h8v, make_uint4(kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]));
         }
-        sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[qat + k * 64], sc[u], 0, 0, 0);
+        sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[qat + (part * QS + k) * 64], sc[u], 0, 0, 0);
       }
     };
-    constexpr bool kBoth = Q4 || HD <= 256;  // both halves of K beside V in registers
-    load_k(0);
-    if constexpr (kBoth) load_k(1);
-    // V: this lane's 8 keys 16 u + 4 g4 + r, some dims of each
-    uint32_t v[8][Q4 ? NH : 4 * NH], dp[4];
+    if constexpr (!kBoth) load_k(cur, 1);
+    scores(0);
+    scores(1);
+    if constexpr (VP == 2) {
+      f4v* xs = reinterpret_cast<f4v*>(lds + HD * 8) + round * (kWaves * 128);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int u = k >> 2, row = row0[u] + 4 * g4 + (k & 3);
-      if constexpr (Q4) {
-        ld_dwords<NH>(vh[u] + (uint32_t)(row * (HD / 2) + part * 128 + c * 4 * NH), v[k]);
-        const uint32_t d = *reinterpret_cast<const uint16_t*>(
-            vh[u] + (uint32_t)((HD / 2 << P.page_shift) + row * (HD / 16) + (part * 8 + c * NH / 4) * 2));
-        dp[k >> 1] = (k & 1) ? dp[k >> 1] | d << 16 : d;
-      } else {
+      for (int u = 0; u < 2; ++u) xs[wave * 128 + u * 64 + lane] = sc[u];
+      lds_sync();
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          uint32_t x[4];
-          ld_dwords<4>(vh[u] + (uint32_t)((row * HD + part * 256 + c * 8 + h * 128) * 2), x);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) v[k][4 * h + t] = x[t];
-        }
-      }
+      for (int u = 0; u < 2; ++u) sc[u] += xs[(wave ^ 1) * 128 + u * 64 + lane];
+      round ^= 1;
     }
     __builtin_amdgcn_sched_barrier(0);
-    scores(0);
-    if constexpr (!kBoth) load_k(1);
-    scores(1);
+    if (more) {  // K's registers are free: the next tile's rows
+      load_k(next, 0);
+      if constexpr (kBoth) load_k(next, 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     // weights
     float p[8], top = kNone;
 #pragma unroll
@@ -229,10 +291,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
         if constexpr (!Q16)  // hi and lo parts of the query
           x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
         x *= scale2;
-        if constexpr (!whole) x = (seen >> (4 * u + r) & 1) ? x : -__builtin_inff();
         p[4 * u + r] = x;
-        top = fmaxf(top, x);
       }
+    if (!whole || cur.there != 3) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) p[k] = (seen >> k & 1) ? p[k] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, p[k]);
     top = quad_max4(top);
     // The maximum is moved where it grows by more than 2^8: until then the
     // weights stay below 2^8 and nothing has to be scaled
@@ -253,82 +319,80 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
       const _Float16 hi = (_Float16)e, lo = (_Float16)(e - (float)hi);
       pf[k] = c < 8 ? hi : lo;
     }
-    // A operands of the dim tiles (h, 0..7): dims 128 h + 8 c + t (f16), 8 NH c + 8 h + t (4 bits) of this
-    // wave's part; the keys whose bit of `mask` is clear count as zeros
-    auto frags = [&](int h, uint32_t mask, h8v(&f)[8]) __attribute__((always_inline)) {
-      uint32_t x[8][4];
+    // Two A operands, of the dim tiles (h, 2 t) and (h, 2 t + 1): dims 128 h + 8 c + .. (f16), 8 NH c + 8 h + ..
+    // (4 bits) of this wave's part; the keys whose bit of `mask` is clear count as zeros
+    auto frags = [&](int h, int t, uint32_t mask, h8v(&f)[2]) __attribute__((always_inline)) {
+      uint32_t x[2][4];
 #pragma unroll
       for (int kp = 0; kp < 4; ++kp) {
         const bool on0 = mask >> (2 * kp) & 1, on1 = mask >> (2 * kp + 1) & 1;
         if constexpr (Q4) {
-          const h2v d2 = h2_of(dp[kp] & ((on0 ? 0xffffu : 0u) | (on1 ? 0xffff0000u : 0u)));
-          h2v e[4], od[4];
-          q4_pairs(lo_halves(v[2 * kp][h], v[2 * kp + 1][h]), e);   // dims 0, 4, 2, 6 of the dword, from bit 0 up
-          q4_pairs(hi_halves(v[2 * kp][h], v[2 * kp + 1][h]), od);  // dims 1, 5, 3, 7
-          constexpr int at[4] = {0, 2, 4, 6};                       // q4_pairs' order: bits 0, 8, 4, 12
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            x[at[t]][kp] = u_of(e[t] * d2);
-            x[at[t] + 1][kp] = u_of(od[t] * d2);
-          }
+          const h2v d2 = h2_of((on0 ? (uint32_t)vd[2 * kp] : 0u) | (on1 ? (uint32_t)vd[2 * kp + 1] << 16 : 0u));
+          // a half of a dword has dims 0, 4, 2, 6 (1, 5, 3, 7) from bit 0 up
+          x[0][kp] = u_of(q4_pair(lo_halves(v[2 * kp][h], v[2 * kp + 1][h]), t) * d2);
+          x[1][kp] = u_of(q4_pair(hi_halves(v[2 * kp][h], v[2 * kp + 1][h]), t) * d2);
         } else {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint32_t a = on0 ? v[2 * kp][4 * h + t] : 0u, b = on1 ? v[2 * kp + 1][4 * h + t] : 0u;
-            x[2 * t][kp] = lo_halves(a, b);
-            x[2 * t + 1][kp] = hi_halves(a, b);
-          }
+          const uint32_t a = on0 ? v[2 * kp][4 * h + t] : 0u, b = on1 ? v[2 * kp + 1][4 * h + t] : 0u;
+          x[0][kp] = lo_halves(a, b);
+          x[1][kp] = hi_halves(a, b);
         }
       }
 #pragma unroll
-      for (int t = 0; t < 8; ++t) f[t] = __builtin_bit_cast(h8v, make_uint4(x[t][0], x[t][1], x[t][2], x[t][3]));
+      for (int e = 0; e < 2; ++e) f[e] = __builtin_bit_cast(h8v, make_uint4(x[e][0], x[e][1], x[e][2], x[e][3]));
     };
     if constexpr (whole) {
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        h8v f[8];
-        frags(h, 0xffu, f);
+      for (int h = 0; h < NH; ++h)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[h][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[k], pf, o[h][k], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+        for (int t = 0; t < 4; ++t) {
+          h8v f[2];
+          frags(h, t, 0xffu, f);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            o[h][2 * t + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[e], pf, o[h][2 * t + e], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
     } else {
       // A row that a token does not see must not reach its output even as 0 x
       // infinity: token by token, with the rows it does not see as zeros
       for (int tok = t_first; tok <= t_last; ++tok) {
         const int pt = s.p0 + tok;
         uint32_t mask = 0;
+        if constexpr (Q4) {  // (what can be unpacked before the loop does not fit in registers)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int h = 0; h < NH; ++h) asm volatile("" : "+v"(v[k][h]));
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int key = kb + 16 * (k >> 2) + 4 * g4 + (k & 3);
-          if (there[k >> 2] && key < cap && key_seen(key, pt, A.window, A.sinks)) mask |= 1u << k;
+          if (key < cap && key_seen(key, pt, A.window, A.sinks)) mask |= 1u << k;
         }
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          h8v f[8];
-          frags(h, mask, f);
+        for (int h = 0; h < NH; ++h)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const f4v x = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[k], pf, f4v{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          for (int t = 0; t < 4; ++t) {
+            h8v f[2];
+            frags(h, t, mask, f);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[h][k][r] += ro.tok == tok ? x[r] : 0.f;
+            for (int e = 0; e < 2; ++e) {
+              const f4v x = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[e], pf, f4v{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[h][2 * t + e][r] += ro.tok == tok ? x[r] : 0.f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
-          __builtin_amdgcn_sched_barrier(0);
-        }
       }
     }
+    if (more) load_v(next);
+    at += W;
   };
-  // Whole tiles, which every row sees all of, then the others: a loop that has
-  // both kept two copies of the output registers
-  auto whole = [&](int kb) {
-    return kb + kPT - 1 <= p_first && (A.window == 0 || kb > p_last - A.window || kb + kPT <= A.sinks) &&
-           paged_page(trow, P.table_stride, P.page_shift, P.n_pages, kb) >= 0 &&
-           paged_page(trow, P.table_stride, P.page_shift, P.n_pages, kb + 16) >= 0;
-  };
-  for (int t = sh.a + stream; t < sh.b; t += W)
-    if (whole(R.base(t))) tile(R.base(t), std::true_type());
-  for (int t = sh.a + stream; t < sh.b; t += W)
-    if (!whole(R.base(t))) tile(R.base(t), std::false_type());
+  while (at < n_whole) tile(std::true_type());
+  while (at < n_all) tile(std::false_type());
+  if constexpr (VP == 2) {  // the streams keep step: as many barriers as the longest one's
+    for (; at - stream < n_all; at += W) lds_sync();
+  }
 
   // the column's sum over the lane groups, the two columns of a row, the waves
   l = quad_sum4(l);
@@ -343,7 +407,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
 #pragma unroll
       for (int t = 0; t < 8; ++t)
         x[t] = o[h][t][r] + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(o[h][t][r]), 0x128, 0xf, 0xf, true));
-      const int dim = 4 * g4 + r, d = part * 256 + (Q4 ? dim * 8 * NH + h * 8 : h * 128 + dim * 8);
+      const int dim = 4 * g4 + r, d = part * HW + (Q4 ? dim * 8 * NH + h * 8 : h * 128 + dim * 8);
       if (c < rows) {
         float* dst = lds + (stream * nr + c) * LD + d;
         *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
@@ -386,27 +450,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   }
 }
 
-// Merge of a row's splits: workgroup (unit, row), HD / 4 threads a split.
-template <int HD>
+// Merge of a row's splits: workgroup (unit, row, DW dims), DW / 4 threads a split
+template <int HD, int DW>
 __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs A) {
-  constexpr int T = HD / 4, NG = 256 / T;
+  constexpr int T = DW / 4, NG = 256 / T;
   __shared__ float wt[kPagedMaxSplits];
   __shared__ float red[4];
-  __shared__ __align__(16) float sum[NG][HD];
+  __shared__ __align__(16) float sum[NG][DW + 4];
   const PagedArgs& P = A.P;
   const int nr = min(A.max_q * A.gqa, kRows);
-  const int r = blockIdx.x % nr, unit = blockIdx.x / nr;
-  const int rb = unit % A.nrb, g = unit / A.nrb % P.kvh, i = unit / A.nrb / P.kvh;
+  const int unit = uni(blockIdx.x / nr), r = blockIdx.x - unit * nr;
+  const int head = uni(unit / A.nrb), rb = unit - head * A.nrb, i = uni(head / P.kvh), g = head - i * P.kvh;
   const SeqSpan s = seq_span(P, i);
   if ((int64_t)s.n * A.gqa > kPagedFewRows) return;
   const int rows = min(min(s.n, A.max_q) * A.gqa - kRows * rb, kRows);
   if (r >= rows) return;
   const int r0 = kRows * rb;
-  const TileRange R = tile_range(s.p0 + r0 / A.gqa, s.p0 + (r0 + rows - 1) / A.gqa, A.window, A.sinks, paged_cap(P));
-  const int live = share_of(R, A.ns, 0, kStreams<HD>).live;
+  const TileRange R = tile_range(s.p0 + uni(r0 / A.gqa), s.p0 + uni((r0 + rows - 1) / A.gqa), A.window, A.sinks, paged_cap(P));
+  const int live = share_of(R, A.ns, 0).live;
   if (live <= 1) return;  // written by its workgroup
-  const int t = threadIdx.x, grp = t / T, d = t % T * 4;
+  const int t = threadIdx.x, grp = t / T, d = blockIdx.y * DW + t % T * 4;
   const int64_t at = (int64_t)unit * A.ns * nr + r;  // + sp * nr
+  float4 y[4];  // the first rounds' loads beside the statistics'
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    y[k] = *reinterpret_cast<const float4*>(A.part + (at + (int64_t)min(grp + k * NG, live - 1) * nr) * HD + d);
   float2 st = make_float2(kNone, 0.f);
   if (t < live) st = *reinterpret_cast<const float2*>(A.part_ml + (at + (int64_t)t * nr) * 2);
   const float M = block_max(st.x, red);
@@ -414,40 +482,48 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs A) {
   if (t < live) wt[t] = f;
   const float L = block_sum(t < live ? f * st.y : 0.f, red);
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int sp = grp; sp < live; sp += NG) {
-    const float4 y = *reinterpret_cast<const float4*>(A.part + (at + (int64_t)sp * nr) * HD + d);
-    const float w = wt[sp];
-    x.x += w * y.x;
-    x.y += w * y.y;
-    x.z += w * y.z;
-    x.w += w * y.w;
-  }
-  *reinterpret_cast<float4*>(&sum[grp][d]) = x;
-  lds_sync();
-  if (grp) return;
+  for (int s0 = grp; s0 < live; s0 += 4 * NG) {
+    float4 z[4];
 #pragma unroll
-  for (int k = 1; k < NG; ++k) {
-    const float4 y = *reinterpret_cast<const float4*>(&sum[k][d]);
-    x.x += y.x;
-    x.y += y.y;
-    x.z += y.z;
-    x.w += y.w;
+    for (int k = 0; k < 4; ++k) z[k] = y[k];
+    if (s0 + 4 * NG < live) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        y[k] = *reinterpret_cast<const float4*>(A.part + (at + (int64_t)min(s0 + (k + 4) * NG, live - 1) * nr) * HD + d);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int sp = s0 + k * NG;
+      if (sp < live) {
+        const float w = wt[sp];
+        x.x += w * z[k].x;
+        x.y += w * z[k].y;
+        x.z += w * z[k].z;
+        x.w += w * z[k].w;
+      }
+    }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<float4*>(&sum[grp][t % T * 4]) = x;
+  lds_sync();
   const RowOf to = row_of(A, g, r0 + r);
-  uint16_t* out = A.out + (int64_t)(s.q0 + to.tok) * A.out_stride + to.head * HD + d;
-  *reinterpret_cast<uint2*>(out) = make_uint2((uint32_t)f2h(x.x * inv) | (uint32_t)f2h(x.y * inv) << 16,
-                                              (uint32_t)f2h(x.z * inv) | (uint32_t)f2h(x.w * inv) << 16);
+  uint16_t* out = A.out + (int64_t)(s.q0 + to.tok) * A.out_stride + to.head * HD + blockIdx.y * DW;
+#pragma unroll
+  for (int j = t; j < DW; j += 256) {
+    float e = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) e += sum[k][j];
+    out[j] = f2h(L == 0.f ? 0.f : e / L);
+  }
 }
 
 template <int HD>
 int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
   constexpr int W = kStreams<HD>;
   const int nr = std::min(a.max_q * a.gqa, kRows), units = a.P.n_seq * a.P.kvh * a.nrb;
-  const size_t lds = std::max((size_t)W * nr * (HD + 4) * 4 + W * kRows * 8, (size_t)HD * 32);
+  const size_t lds = std::max((size_t)W * nr * (HD + 4) * 4 + W * kRows * 8, (size_t)HD * 32 + (kParts<HD> == 2 ? 2 * kWaves * 128 * 16 : 0));
   const dim3 grid((unsigned)(units * a.ns));
   auto go = [&](auto* kernel) {
-    // (more than 64 KB of LDS has to be asked for; 68.1 KB at most here)
+    // (more than 64 KB of LDS has to be asked for; 67 KB at most here)
     if (lds > 65536)
       E4B_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     kernel<<<grid, 64 * kWaves, lds, st>>>(a);
@@ -459,21 +535,24 @@ int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
            : q16     ? go(k_attn_paged_few<HD, false, true>)
                      : go(k_attn_paged_few<HD, false, false>);
   if (rc || a.ns == 1) return rc;
-  k_attn_paged_merge<HD><<<units * nr, 256, 0, st>>>(a);
+  // a few rows: more workgroups a row, each with fewer splits to add up in turn
+  if (units * nr < 128)
+    k_attn_paged_merge<HD, 64><<<dim3(units * nr, HD / 64), 256, 0, st>>>(a);
+  else
+    k_attn_paged_merge<HD, HD><<<units * nr, 256, 0, st>>>(a);
   E4B_HIP(hipGetLastError());
   return E4B_OK;
 }
 
 }  // namespace
 
-void plan_attn_paged_few(PagedAttnArgs& a, int hd) {
-  const int W = hd == 512 ? kStreams<512> : kStreams<256>;
+void plan_attn_paged_few(PagedAttnArgs& a, int hd, bool q4) {
   a.nrb = (a.max_q * a.gqa + kRows - 1) / kRows;
   const int64_t units = (int64_t)a.P.n_seq * a.P.kvh * a.nrb;
   const int64_t seen = a.window ? std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + a.max_q) : a.max_kv;
   const int64_t tiles = seen / kPT + 2;
-  int64_t ns = std::min<int64_t>((512 + units - 1) / units, tiles / W);
-  if (tiles <= 2 * W) ns = 1;
+  int64_t ns = std::min<int64_t>(kMaxGroups / units, (tiles + kMinShare - 1) / kMinShare);
+  if (tiles <= kUnsplit) ns = 1;
   a.ns = (int)std::max<int64_t>(1, std::min<int64_t>(ns, kPagedMaxSplits));
   const int nr = std::min(a.max_q * a.gqa, kRows);
   a.part_floats = a.ns > 1 ? (size_t)units * a.ns * nr * hd : 0;

@@ -120,7 +120,7 @@ struct PagedAttnArgs {
   float* part_ml;
 };
 // a few query rows per sequence and KV head (k_paged_decode.hip)
-void plan_attn_paged_few(PagedAttnArgs& a, int hd);
+void plan_attn_paged_few(PagedAttnArgs& a, int hd, bool q4);
 int launch_attn_paged_few(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
 constexpr int kPagedFewRows = 16;  // most rows of a sequence and KV head that it takes
 // any number (k_paged_chunk.hip)

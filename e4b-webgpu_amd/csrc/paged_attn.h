@@ -37,24 +37,21 @@ DEV bool key_seen(int key, int pos, int window, int sinks) {
   return key <= pos && (window == 0 || key > pos - window || key < sinks);
 }
 
-// eight codes of a dword as f16 values (code - 8) d, dims in order; d2 = (d, d).
-// A half 0x6400 | n is 1024 + n, one with n four bits up 1024 + 16 n: taking
+// Codes of a dword as f16 values: a pair of halves (code - 8), and all eight
+// (code - 8) d with dims in order, d2 = (d, d).  A half 0x6400 | n is 1024 + n, one with n four bits up 1024 + 16 n: taking
 // 1032 off, or 1/16 of it less 72, is exact.
-DEV void q4_pairs(uint32_t w, h2v (&p)[4]) {
-  const uint32_t w8 = w >> 8, one = 0x64006400u, lo = 0x000F000Fu, hi = 0x00F000F0u;
+DEV h2v q4_pair(uint32_t w, int i) {  // pair i = 0 .. 3, at bits 0, 8, 4, 12
   const h2v c = {(_Float16)1032.f, (_Float16)1032.f}, s = {(_Float16)0.0625f, (_Float16)0.0625f},
             e = {(_Float16)72.f, (_Float16)72.f};
-  p[0] = __builtin_bit_cast(h2v, (w & lo) | one) - c;
-  p[1] = __builtin_bit_cast(h2v, (w8 & lo) | one) - c;
-  p[2] = __builtin_elementwise_fma(__builtin_bit_cast(h2v, (w & hi) | one), s, -e);
-  p[3] = __builtin_elementwise_fma(__builtin_bit_cast(h2v, (w8 & hi) | one), s, -e);
+  const uint32_t x = i & 1 ? w >> 8 : w;
+  if (i < 2) return __builtin_bit_cast(h2v, (x & 0x000F000Fu) | 0x64006400u) - c;
+  return __builtin_elementwise_fma(__builtin_bit_cast(h2v, (x & 0x00F000F0u) | 0x64006400u), s, -e);
 }
 DEV h2v h2_of(uint32_t w) { return __builtin_bit_cast(h2v, w); }
 DEV uint32_t u_of(h2v v) { return __builtin_bit_cast(uint32_t, v); }
 DEV h8v q4_frag(uint32_t w, h2v d2) {
-  h2v p[4];
-  q4_pairs(w, p);
-  return __builtin_bit_cast(h8v, make_uint4(u_of(p[0] * d2), u_of(p[1] * d2), u_of(p[2] * d2), u_of(p[3] * d2)));
+  return __builtin_bit_cast(h8v, make_uint4(u_of(q4_pair(w, 0) * d2), u_of(q4_pair(w, 1) * d2), u_of(q4_pair(w, 2) * d2),
+                                            u_of(q4_pair(w, 3) * d2)));
 }
 // halves 0 or 1 of two dwords side by side
 DEV uint32_t lo_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
