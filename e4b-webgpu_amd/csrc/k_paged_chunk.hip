@@ -49,19 +49,14 @@ DEV TileAt find_tile(const PagedAttnArgs& A, int rows_per, int at) {
       const int rows = (min(max(A.P.q_start[b + lane + 1], q0), A.P.n_tok) - q0) * A.gqa;
       n = rows <= A.few_rows ? 0 : (rows + rows_per - 1) / rows_per;
     }
-    int upto = n;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int x = __shfl_up(upto, m, 64);
-      if (lane >= m) upto += x;
-    }
+    const int upto = wave_scan(n);
     const uint64_t past = __ballot(at < upto);
     if (past) {
       const int f = __builtin_ctzll(past);
       const int last = __builtin_amdgcn_readlane(upto, f) - 1 - at;
       return {b + f, last};
     }
-    at -= __builtin_amdgcn_readlane(upto, 63);
+    at -= last_lane(upto);
   }
   return {-1, 0};
 }

@@ -39,28 +39,154 @@ constexpr int kParts = HD / 256 > 1 ? 2 : 1;
 template <int HD>
 constexpr int kStreams = kWaves / kParts<HD>;  // tiles at a time in a workgroup
 
-// row c of a unit: token and head
+// Splits.  A workgroup fills a CU, so there are about as many as CUs (one
+// token at 32767 positions in 4 bits 15.7 us with 256 workgroups, 21.2 with
+// 512), dealt out by the sequences' lengths.  A split is a launch more (about
+// 4 us), and what it saves is the time in which one CU takes in its share: none
+// up to 7 tiles (one token at 128 positions 7.2 us in one workgroup, 9.0 in
+// two), shares of 4 tiles above (at 300 positions 10.6 us, 12.9 in one
+// workgroup; shares of 2 10.7 us).
+constexpr int kMinShare = 4, kUnsplit = 7, kGroups = 256;
+constexpr int kSplitSeqs = 256;  // sequences whose lengths a workgroup looks through
+
+// rows and key tiles of block rb of sequence i (any i: by lanes)
+struct Block {
+  SeqSpan s;
+  int rows, t_first, t_last;  // its tokens
+  TileRange R;
+};
+DEV Block block_of(const PagedAttnArgs& A, const SeqSpan& s, int rb, int cap) {
+  Block b;
+  b.s = s;
+  b.rows = (int64_t)s.n * A.gqa > kPagedFewRows ? 0  // k_paged_chunk.hip's
+                                                : max(0, min(min(s.n, A.max_q) * A.gqa - kRows * rb, kRows));
+  b.t_first = rb ? A.second : 0;
+  b.t_last = max(b.t_first, min(s.n - 1, rb ? A.last[1] : A.last[0]));
+  b.R = tile_range(s.p0 + b.t_first, s.p0 + b.t_last, A.window, A.sinks, cap);
+  return b;
+}
+
+// A unit (sequence, block of rows, KV head), and of its `live` splits number
+// sp, the workgroup `first` + sp
+struct Slot {
+  int seq, rb, head, sp, live, first;
+  SeqSpan s;
+};
+// Without splits workgroup and unit are the same.  Else a unit has a split for
+// each `per` tiles (and takes even shares of its tiles), per being as small as
+// leaves no more than A.groups workgroups in all, from the lengths of all
+// sequences (a lane a sequence, 64 at a time; 131072 units at most).  The slot of workgroup `at`, or (by
+// unit) of the unit `at` with sp = 0; seq < 0: there is none.
+DEV int quotient(int a, int b) {  // a / b for a < 2^21: the error of (a + 1/2) / b in f32 is below 1 / (2 b)
+  return uni((int)(((float)a + 0.5f) / (float)b));
+}
+DEV Slot find_slot(const PagedAttnArgs& A, int at, bool by_unit) {
+  const PagedArgs& P = A.P;
+  if (!A.split) {
+    const int u = uni(at / A.nrb), i = uni(u / P.kvh);
+    return {i, at - u * A.nrb, u - i * P.kvh, 0, 1, at, seq_span(P, i)};
+  }
+  constexpr int NC = kSplitSeqs / 64, NB = (kPagedFewRows + kRows - 1) / kRows;
+  const int lane = threadIdx.x & 63, cap = paged_cap(P);
+  int tiles[NC][NB];  // -1: no such block
+  int start[NC], end[NC], kv[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) tiles[c][b] = -1;
+  int sum = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    if (64 * c < P.n_seq) {
+      const int i = min(64 * c + lane, P.n_seq - 1);
+      start[c] = P.q_start[i];
+      end[c] = P.q_start[i + 1];
+      kv[c] = P.kv_len[i];
+      const SeqSpan s = seq_span_of(P, start[c], end[c], kv[c]);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const Block k = block_of(A, s, b, cap);
+        if (64 * c + lane < P.n_seq && k.rows > 0) tiles[c][b] = k.R.n;
+        sum += max(tiles[c][b], 0);
+      }
+    }
+  // (t / per rounded up, or one more or less: every workgroup finds the same)
+  auto splits = [&](int t, float by) {
+    return t < 0 ? 0 : t <= kUnsplit ? 1 : max(1, min((int)((float)t * by + 0.999f), kPagedMaxSplits));
+  };
+  auto all = [&](float by) {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (64 * c < P.n_seq)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) n += splits(tiles[c][b], by);
+    return last_lane(wave_scan(n)) * P.kvh;
+  };
+  const float share = (float)last_lane(wave_scan(min(sum, 1 << 24))) * (float)P.kvh / (float)A.target;
+  float by = 1.f / fmaxf((float)kMinShare, share);  // splits a tile
+#pragma unroll 1
+  for (int k = 0; k < 4; ++k) {
+    const int n = all(by);
+    if (n <= A.groups) break;
+    by = k == 3 ? 0.f : by * 0.99f * (float)A.groups / (float)n;
+  }
+  int before = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    if (64 * c < P.n_seq) {
+      int n = 0;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) n += splits(tiles[c][b], by);
+      const int upto = before + wave_scan(n) * P.kvh;
+      int f;
+      if (by_unit) {
+        const int i = quotient(at, A.nrb * P.kvh);
+        if (i >= 64 * (c + 1)) {
+          before = last_lane(upto);
+          continue;
+        }
+        f = i - 64 * c;
+      } else {
+        const uint64_t past = __ballot(at < upto);
+        if (!past) {
+          before = last_lane(upto);
+          continue;
+        }
+        f = __builtin_ctzll(past);
+      }
+      Slot r{64 * c + f, 0, 0, 0, 0, __builtin_amdgcn_readlane(upto - n * P.kvh, f),
+             seq_span_of(P, __builtin_amdgcn_readlane(start[c], f), __builtin_amdgcn_readlane(end[c], f),
+                         __builtin_amdgcn_readlane(kv[c], f))};
+      const int i = by_unit ? at - r.seq * A.nrb * P.kvh : 0;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int live = __builtin_amdgcn_readlane(splits(tiles[c][b], by), f);
+        r.rb = b;
+        r.live = live;
+        if (by_unit) {
+          if ((A.nrb == 2 ? i & 1 : 0) == b) {
+            r.head = A.nrb == 2 ? i >> 1 : i;
+            r.first += r.head * live;
+            return r;
+          }
+        } else if (at < r.first + live * P.kvh) {
+          r.head = quotient(at - r.first, live);
+          r.first += r.head * live;
+          r.sp = at - r.first;
+          return r;
+        }
+        r.first += live * P.kvh;
+      }
+    }
+  return {-1, 0, 0, 0, 0, 0, {}};
+}
+
+// row r of a unit: token and head
 struct RowOf {
   int tok, head;
 };
 DEV RowOf row_of(const PagedAttnArgs& A, int g, int r) { return {r / A.gqa, g * A.gqa + r % A.gqa}; }
-
-// Splits.  A workgroup fills a CU, so there are at most as many as CUs (one
-// token at 32767 positions in 4 bits 15.7 us with 256 workgroups, 21.2 with
-// 512).  A split is a launch more (about 4 us), and what it saves is the time
-// in which one CU takes in its share: none up to 7 tiles (one token at 128
-// positions 7.2 us in one workgroup, 9.0 in two), shares of 4 tiles above (at
-// 300 positions 10.6 us, 12.9 in one workgroup; shares of 2 10.7 us).
-constexpr int kMinShare = 4, kUnsplit = 7, kMaxGroups = 256;
-
-// the share of split sp: tiles a .. b - 1
-struct Share {
-  int a, b, live;  // live: splits that have any
-};
-DEV Share share_of(const TileRange& R, int ns, int sp) {
-  const int per = max(kMinShare, uni((R.n + ns - 1) / ns));
-  return {min(sp * per, R.n), min((sp + 1) * per, R.n), uni((R.n + per - 1) / per)};
-}
 
 // what a page that is not there is read as (never written): codes of a page
 // and 16 rows' scales, or 16 rows, whichever is more
@@ -91,18 +217,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   const PagedArgs& P = A.P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g4 = lane >> 4;
-  const int unit = uni(blockIdx.x / A.ns), sp = blockIdx.x - unit * A.ns;
-  const int head = uni(unit / A.nrb), rb = unit - head * A.nrb, i = uni(head / P.kvh), g = head - i * P.kvh;
-  const SeqSpan s = seq_span(P, i);
-  if ((int64_t)s.n * A.gqa > kPagedFewRows) return;  // k_paged_chunk.hip's
-  const int rows = min(min(s.n, A.max_q) * A.gqa - kRows * rb, kRows);
-  if (rows <= 0) return;
+  const Slot slot = find_slot(A, blockIdx.x, false);
+  const int i = uni(slot.seq), g = uni(slot.head), rb = uni(slot.rb), sp = uni(slot.sp), live = uni(slot.live);
+  if (i < 0) return;
   const int cap = paged_cap(P);
-  const int r0 = kRows * rb, t_first = uni(r0 / A.gqa), t_last = uni((r0 + rows - 1) / A.gqa);
+  const Block blk = block_of(A, slot.s, rb, cap);
+  const SeqSpan& s = blk.s;
+  const int rows = blk.rows, r0 = kRows * rb, t_first = uni(blk.t_first), t_last = uni(blk.t_last);
+  if (rows <= 0) return;
   const int p_first = s.p0 + t_first, p_last = s.p0 + t_last;
   const TileRange R = tile_range(p_first, p_last, A.window, A.sinks, cap);
-  const Share sh = share_of(R, A.ns, sp);
-  if (sh.a >= sh.b && !(sp == 0 && R.n == 0)) return;
+  const bool whole_unit = live <= 1;
+  const int per = uni((R.n + max(live, 1) - 1) / max(live, 1));
+  const int sha = min(sp * per, R.n), shb = min((sp + 1) * per, R.n);
   const RowOf ro = row_of(A, g, r0 + min(c & 7, rows - 1));
   const int pos = s.p0 + ro.tok;  // of this lane's column
   const table_ptr trow = table_row(P, i);
@@ -113,10 +240,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   const int stream = wave / VP, part = wave % VP;  // part: the wave's dims are HW part ..
   const int wa = R.sink - R.from + (A.window > 0 ? max(0, p_last - A.window + kPT) / kPT : 0);
   const int wb = R.sink - R.from + max(0, min(p_first, cap - 1) + 1) / kPT;
-  const int a0 = min(max(sh.a, wa), sh.b), n_whole = max(0, min(sh.b, wb) - a0), n_all = sh.b - sh.a;
+  const int a0 = min(max(sha, wa), shb), n_whole = max(0, min(shb, wb) - a0), n_all = shb - sha;
   auto base_of = [&](int v) {
-    const int before = a0 - sh.a, e = v - n_whole;
-    return R.base(v < n_whole ? a0 + v : e < before ? sh.a + e : v + sh.a);
+    const int before = a0 - sha, e = v - n_whole;
+    return R.base(v < n_whole ? a0 + v : e < before ? sha + e : v + sha);
   };
   // A tile's halves: their pages' blocks and the first rows there.  A half
   // without a page is read from zeros.
@@ -436,14 +563,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
       x.z += f * y.z;
       x.w += f * y.w;
     }
-    if (sh.live <= 1) {
+    if (whole_unit) {
       const float inv = L == 0.f ? 0.f : 1.f / L;
       const RowOf to = row_of(A, g, r0 + r);
       uint16_t* out = A.out + (int64_t)(s.q0 + to.tok) * A.out_stride + to.head * HD + d;
       *reinterpret_cast<uint2*>(out) = make_uint2((uint32_t)f2h(x.x * inv) | (uint32_t)f2h(x.y * inv) << 16,
                                                   (uint32_t)f2h(x.z * inv) | (uint32_t)f2h(x.w * inv) << 16);
     } else {
-      const int64_t at = ((int64_t)unit * A.ns + sp) * nr + r;
+      const int64_t at = (int64_t)blockIdx.x * nr + r;
       *reinterpret_cast<float4*>(A.part + at * HD + d) = x;
       if (d == 0) *reinterpret_cast<float2*>(A.part_ml + at * 2) = make_float2(M, L);
     }
@@ -460,23 +587,20 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs A) {
   const PagedArgs& P = A.P;
   const int nr = min(A.max_q * A.gqa, kRows);
   const int unit = uni(blockIdx.x / nr), r = blockIdx.x - unit * nr;
-  const int head = uni(unit / A.nrb), rb = unit - head * A.nrb, i = uni(head / P.kvh), g = head - i * P.kvh;
-  const SeqSpan s = seq_span(P, i);
-  if ((int64_t)s.n * A.gqa > kPagedFewRows) return;
-  const int rows = min(min(s.n, A.max_q) * A.gqa - kRows * rb, kRows);
-  if (r >= rows) return;
+  const Slot slot = find_slot(A, unit, true);
+  const int i = uni(slot.seq), g = uni(slot.head), rb = uni(slot.rb), live = uni(slot.live);
+  if (i < 0 || live <= 1) return;  // written by its workgroup
+  const SeqSpan s = slot.s;
   const int r0 = kRows * rb;
-  const TileRange R = tile_range(s.p0 + uni(r0 / A.gqa), s.p0 + uni((r0 + rows - 1) / A.gqa), A.window, A.sinks, paged_cap(P));
-  const int live = share_of(R, A.ns, 0).live;
-  if (live <= 1) return;  // written by its workgroup
+  if (r >= block_of(A, s, rb, paged_cap(P)).rows) return;
   const int t = threadIdx.x, grp = t / T, d = blockIdx.y * DW + t % T * 4;
-  const int64_t at = (int64_t)unit * A.ns * nr + r;  // + sp * nr
+  const int64_t at = (int64_t)slot.first * nr + r;  // + sp * nr
   float4 y[4];  // the first rounds' loads beside the statistics'
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     y[k] = *reinterpret_cast<const float4*>(A.part + (at + (int64_t)min(grp + k * NG, live - 1) * nr) * HD + d);
   float2 st = make_float2(kNone, 0.f);
-  if (t < live) st = *reinterpret_cast<const float2*>(A.part_ml + (at + (int64_t)t * nr) * 2);
+  if (t < live) st = *reinterpret_cast<const float2*>(A.part_ml + (at + (int64_t)t * nr) * 2);  // (live <= kGroups)
   const float M = block_max(st.x, red);
   const float f = exp2_(st.x - M);
   if (t < live) wt[t] = f;
@@ -521,7 +645,7 @@ int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
   constexpr int W = kStreams<HD>;
   const int nr = std::min(a.max_q * a.gqa, kRows), units = a.P.n_seq * a.P.kvh * a.nrb;
   const size_t lds = std::max((size_t)W * nr * (HD + 4) * 4 + W * kRows * 8, (size_t)HD * 32 + (kParts<HD> == 2 ? 2 * kWaves * 128 * 16 : 0));
-  const dim3 grid((unsigned)(units * a.ns));
+  const dim3 grid((unsigned)a.groups);
   auto go = [&](auto* kernel) {
     // (more than 64 KB of LDS has to be asked for; 67 KB at most here)
     if (lds > 65536)
@@ -534,7 +658,7 @@ int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
            : q4      ? go(k_attn_paged_few<HD, true, false>)
            : q16     ? go(k_attn_paged_few<HD, false, true>)
                      : go(k_attn_paged_few<HD, false, false>);
-  if (rc || a.ns == 1) return rc;
+  if (rc || !a.split) return rc;
   // a few rows: more workgroups a row, each with fewer splits to add up in turn
   if (units * nr < 128)
     k_attn_paged_merge<HD, 64><<<dim3(units * nr, HD / 64), 256, 0, st>>>(a);
@@ -546,17 +670,22 @@ int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
 
 }  // namespace
 
-void plan_attn_paged_few(PagedAttnArgs& a, int hd, bool q4) {
+void plan_attn_paged_few(PagedAttnArgs& a, int hd) {
   a.nrb = (a.max_q * a.gqa + kRows - 1) / kRows;
-  const int64_t units = (int64_t)a.P.n_seq * a.P.kvh * a.nrb;
+  const int units = a.P.n_seq * a.P.kvh * a.nrb;
   const int64_t seen = a.window ? std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + a.max_q) : a.max_kv;
   const int64_t tiles = seen / kPT + 2;
-  int64_t ns = std::min<int64_t>(kMaxGroups / units, (tiles + kMinShare - 1) / kMinShare);
-  if (tiles <= kUnsplit) ns = 1;
-  a.ns = (int)std::max<int64_t>(1, std::min<int64_t>(ns, kPagedMaxSplits));
+  // Where the units fill the CUs, splitting is for lengths that differ: from
+  // 2048 keys on
+  a.split = a.P.n_seq <= kSplitSeqs && (units < kGroups ? tiles > kUnsplit : tiles > 64);
+  a.second = kRows / a.gqa;
+  a.last[0] = (kRows - 1) / a.gqa;
+  a.last[1] = (2 * kRows - 1) / a.gqa;
+  a.target = std::max(units, kGroups);
+  a.groups = !a.split ? units : units < kGroups ? kGroups : 2 * units;
   const int nr = std::min(a.max_q * a.gqa, kRows);
-  a.part_floats = a.ns > 1 ? (size_t)units * a.ns * nr * hd : 0;
-  a.ml_floats = a.ns > 1 ? (size_t)units * a.ns * nr * 2 : 0;
+  a.part_floats = a.split ? (size_t)a.groups * nr * hd : 0;
+  a.ml_floats = a.split ? (size_t)a.groups * nr * 2 : 0;
 }
 
 int launch_attn_paged_few(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st) {

@@ -58,15 +58,17 @@ typedef const __attribute__((address_space(4))) int32_t* lens_ptr;
 DEV table_ptr table_row(const PagedArgs& P, int i) {
   return (table_ptr)(uintptr_t)P.table + (int64_t)i * P.table_stride;
 }
-DEV SeqSpan seq_span(const PagedArgs& P, int i) {
+DEV SeqSpan seq_span_of(const PagedArgs& P, int start, int end, int kv) {
   SeqSpan s;
-  const lens_ptr q_start = (lens_ptr)(uintptr_t)P.q_start, kv_len = (lens_ptr)(uintptr_t)P.kv_len;
-  const int a = q_start[i], b = q_start[i + 1];
-  s.q0 = min(max(a, 0), P.n_tok);
-  s.n = min(max(b, s.q0), P.n_tok) - s.q0;
-  s.kv = max(kv_len[i], 0);
+  s.q0 = min(max(start, 0), P.n_tok);
+  s.n = min(max(end, s.q0), P.n_tok) - s.q0;
+  s.kv = max(kv, 0);
   s.p0 = s.kv - s.n;
   return s;
+}
+DEV SeqSpan seq_span(const PagedArgs& P, int i) {
+  const lens_ptr q_start = (lens_ptr)(uintptr_t)P.q_start, kv_len = (lens_ptr)(uintptr_t)P.kv_len;
+  return seq_span_of(P, q_start[i], q_start[i + 1], kv_len[i]);
 }
 // the sequence of token t (n_seq: behind the last one); the whole wave calls it
 DEV int seq_of_token(const PagedArgs& P, int t) {
@@ -101,7 +103,7 @@ struct KvAppendArgs {
 int launch_kv_append(const KvAppendArgs& a, int hd, bool q4, bool x16, hipStream_t st);
 int launch_kv_gather(const PagedArgs& P, int hd, bool q4, uint16_t* k_out, uint16_t* v_out, hipStream_t st);
 
-constexpr int kPagedMaxSplits = 256;
+constexpr int kPagedMaxSplits = 256;  // of a unit with few rows
 struct PagedAttnArgs {
   PagedArgs P;
   const void* q;            // f32 or f16 rows of qh heads
@@ -114,13 +116,16 @@ struct PagedAttnArgs {
   // the plan: blocks of rows (tokens x heads of a group) of a sequence, splits
   // of the keys, and where the splits' results go
   int nrb, ns;
+  int groups, target;       // few rows: workgroups, and how many the key tiles are cut for
+  bool split;
+  int second, last[2];      // first token of the second block of 8 rows, last ones of both
   int few_rows;             // chunks: sequences with no more rows than this are left out
   size_t part_floats, ml_floats;
   float* part;
   float* part_ml;
 };
 // a few query rows per sequence and KV head (k_paged_decode.hip)
-void plan_attn_paged_few(PagedAttnArgs& a, int hd, bool q4);
+void plan_attn_paged_few(PagedAttnArgs& a, int hd);
 int launch_attn_paged_few(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
 constexpr int kPagedFewRows = 16;  // most rows of a sequence and KV head that it takes
 // any number (k_paged_chunk.hip)

@@ -175,7 +175,7 @@ static int attn_setup(const char* fn, const e4b_paged_kv* kv, const e4b_kv_batch
   if (plan->use_few) {
     plan->few = a;
     plan->few.max_q = std::min(a.max_q, kPagedFewRows / a.gqa);
-    plan_attn_paged_few(plan->few, kv->head_dim, kv->type == E4B_KV_Q4);
+    plan_attn_paged_few(plan->few, kv->head_dim);
   }
   if (plan->use_chunk) {
     plan->chunk = a;

@@ -14,6 +14,18 @@ constexpr int kPT = 32;  // keys per tile: two 16-key halves, each inside one pa
 // division leaves it in a vector one, and what depends on it with it)
 DEV int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// sums over the lanes up to this one
+DEV int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: inside 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the last lane of 16 to the next 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // and of 32 to the next 32
+  return v;
+}
+DEV int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+
 // Tiles of the keys that queries at positions p0 .. p1 see, in the order of
 // the keys: `sink` tiles from 0 on, then the ones from `from` on.
 struct TileRange {
