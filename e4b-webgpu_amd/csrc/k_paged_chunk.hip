@@ -10,8 +10,18 @@
 //   S^T (16 keys x 16 columns) = K . Q^T, K read row by row;
 //   O^T (16 dims x 16 columns) += V^T . P^T, V^T read with the transposing
 //   ds_read_b64_tr_b16, P as it lies in the registers after the softmax.
-// A fragment of K or V (1 KB of LDS reads) feeds F products: with F = 2 the
-// LDS's 128 bytes a clock and the matrix units' rate are matched.
+// A fragment of K or V (1 KB of LDS reads) feeds F products.
+//
+// What bounds it: the matrix units work for 40 % of the kernel's time and the
+// waves issue for most of the rest -- the softmax's exponentials and
+// conversions are 16 values a lane and tile beside 32 products, and 256
+// registers a wave leave two waves a SIMD to hide them behind each other.  At
+// head dim 256, 4 query heads a KV head, f16 queries: 8 sequences of 1024
+// tokens at 4096 positions 257 us (0.94 PFLOP/s), 16 of them 504; 4 sequences
+// with f32 queries 277 (each product twice); 4 bits 8 sequences 367 (a tile is
+// turned into f16 by each workgroup that reads it).  Wider and narrower tiles
+// (F 1 with 8 waves, F 1 with 4) were 1.1 to 1.4 times slower: fewer products
+// for each fragment that LDS delivers.
 #include <algorithm>
 
 #include "../../include/e4b.h"
@@ -79,23 +89,36 @@ DEV float cache_value(const uint8_t* block, int row, int d, int page_shift) {
   }
 }
 
-// 16-byte piece `p` of row r of a tile in LDS: rows are whole bank rounds
-// apart, so the pieces are moved by the row (K: 16 rows are read at once, V:
-// 16 rows of 32 bytes)
-template <int HD>
-DEV int k_piece(int r, int p) { return p ^ (r & 15); }
-template <int HD>
-DEV int v_piece(int r, int p) { return p ^ ((r & (HD == 128 ? 7 : 15)) << 1); }
+// 16-byte piece `p` of row r (of 16) of a tile in LDS.  Rows are whole rounds of
+// the banks apart, so the pieces are moved by the row: the 16 rows of a K
+// fragment to 16 places, and of a V fragment (two pieces side by side of each
+// row, 8 rows at a time) to 8 pairs of places.
+DEV int piece(int r, int p) { return p ^ ((r & 7) << 1 | (r >> 3 & 1)); }
 
 template <int HD, bool Q4, bool Q16>
 __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(PagedAttnArgs A) {
   constexpr int F = kFrags<HD>, NW = kChunkWaves<HD>, BM = kTileRows<HD, Q16>, RF = Q16 ? 16 : 8;
+  // fragments of K and V that are read ahead of their products; 4-bit tiles need
+  // the registers on their way (f32 queries of f16 310 us with 2, 301 with 3;
+  // 8 sequences of 4 bits 380 and 390)
+  constexpr int kAhead = Q4 ? 2 : 3, kAheadV = Q4 ? 2 : 3;
   constexpr int QS = HD / 32, DT = HD / 16, KP = HD / 8, TP = kPT * KP;  // TP: 16-byte pieces of a K or V tile
-  __shared__ __align__(16) uint4 bufs[2][2 * TP];
+  // two buffers of a K and a V tile, and the mark of a broken cache.  One array:
+  // beside a second LDS variable the compiler drops what it knows of the two
+  // buffers (below) and waits for the copies into one at each read of the other.
+  __shared__ __align__(16) uint4 lds[4 * TP + 1];
+  auto buf_of = [&](int n) { return lds + (n & 1) * 2 * TP; };
+  uint32_t* mark = reinterpret_cast<uint32_t*>(lds + 4 * TP);
   const PagedArgs& P = A.P;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g4 = lane >> 4;
-  const int sp = blockIdx.x % A.ns, g = blockIdx.x / A.ns % P.kvh, at = blockIdx.x / A.ns / P.kvh;
+  // Workgroups n and n + 256 share a CU while the first 512 start, and tiles go
+  // from the most keys to the fewest along a sequence: the second 256 in
+  // reverse put long beside short (8 x 1024 tokens at 4096 positions: 267 us
+  // without, 257 with; 8 ragged prompts of up to 2048 tokens: 126 and 132).
+  int unit = blockIdx.x;
+  if (unit >> 8 == 1) unit = 256 + min(512, (int)gridDim.x) - 1 - unit;
+  const int sp = unit % A.ns, g = unit / A.ns % P.kvh, at = unit / A.ns / P.kvh;
   const TileAt ta = find_tile(A, BM, at);
   const int i = __builtin_amdgcn_readfirstlane(ta.seq), qt = __builtin_amdgcn_readfirstlane(ta.tile);
   if (i < 0) return;
@@ -108,7 +131,6 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
   const int per = chunk_per(R.n, A.ns), live = uni((R.n + per - 1) / per);  // tiles of a split, splits that have any
   const int n_tiles = max(0, min(per, R.n - sp * per)), first = sp * per;
   if (n_tiles == 0 && !(sp == 0 && R.n == 0)) return;
-  const table_ptr trow = table_row(P, i);
 
   // this wave's rows, and this lane's column of each fragment
   const int w0 = t0 + wave * F * RF, w1 = min(w0 + F * RF, t1);
@@ -130,47 +152,56 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
     int row;
     bool there;
   };
-  auto half_at = [&](int kb, int u) {
-    const int p = kb + 16 * u, b = p >> P.page_shift;
-    const uint32_t pg = trow[min(b, P.table_stride - 1)];
-    const bool there = b < P.table_stride && pg < (uint32_t)P.n_pages;
+  // The table's entries for a tile are asked for two tiles ahead, with vector
+  // loads that come back in order with the rows': no wait of their own.
+  const uint32_t* tab = P.table + (int64_t)i * P.table_stride;
+  auto ask = [&](int n, uint32_t(&pg)[2]) __attribute__((always_inline)) {
+    const int kb = R.base(first + min(n, n_tiles - 1));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) pg[u] = tab[min((kb + 16 * u) >> P.page_shift, P.table_stride - 1)];
+  };
+  auto half_of = [&](int kb, int u, uint32_t entry) __attribute__((always_inline)) {
+    const int p = kb + 16 * u;
+    const uint32_t pg = uni(entry);
+    const bool there = (p >> P.page_shift) < P.table_stride && pg < (uint32_t)P.n_pages;
     const int64_t blk = paged_block<Q4, HD>(P, there ? (int)pg : 0, g);
     return Half{P.k + blk, P.v + blk, p & ((1 << P.page_shift) - 1), there};
+  };
+  auto second_half = [&](Half h, int kb, uint32_t entry) __attribute__((always_inline)) {
+    if (P.page_shift < 5) return half_of(kb, 1, entry);
+    h.row += 16;  // both halves of a tile are in one page
+    return h;
   };
   // f16: rows go straight into LDS, 1 KB a wave at a time
   constexpr int RI = 1024 / (2 * HD);             // rows of a copy
   constexpr int HC = 16 / RI / NW;                // copies of a wave for a half of K or V
   static_assert(HC * NW * RI == 16, "the waves share a half evenly");
-  int at_k[HC], at_v[HC];
+  int from[HC];
 #pragma unroll
   for (int j = 0; j < HC; ++j) {
     const int r = (j * NW + wave) * RI + lane / KP, p = lane % KP;
-    at_k[j] = r * (2 * HD) + k_piece<HD>(r, p) * 16;
-    at_v[j] = r * (2 * HD) + v_piece<HD>(r, p) * 16;
+    from[j] = r * (2 * HD) + piece(r, p) * 16;
   }
   auto copy16 = [](const uint8_t* base, uint4* dst, int lane_off, int off) __attribute__((always_inline)) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0xffffffffu, 0x00020000), (lds_void*)dst, 16, lane_off, off, 0, 0);
   };
-  auto copy = [&](uint4* buf, int kb) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const Half H = half_at(kb, u);
-#pragma unroll
-      for (int j = 0; j < HC; ++j) {
-        uint4* dst = buf + u * 16 * KP + (j * NW + wave) * 64;
-        copy16(H.k, dst, at_k[j], H.row * (2 * HD));
-        copy16(H.v, dst + TP, at_v[j], H.row * (2 * HD));
-      }
-    }
+  constexpr int NC = 4 * HC;  // copies of a wave for a tile
+  auto copy = [&](uint4* buf, Half H0, Half H1, int n) __attribute__((always_inline)) {  // number n of them
+    const int u = n / HC % 2, j = n % HC;
+    const Half H = u ? H1 : H0;
+    uint4* dst = buf + u * 16 * KP + (j * NW + wave) * 64;
+    if (n < 2 * HC)
+      copy16(H.k, dst, from[j], H.row * (2 * HD));
+    else
+      copy16(H.v, dst + TP, from[j], H.row * (2 * HD));
   };
   // 4 bits: a thread takes 32 dims of a row (16 bytes of codes and their
   // scale) into registers one tile ahead and writes them to LDS as f16
   constexpr int ST = 2 * kPT * (HD / 32) / (64 * NW);  // blocks of a thread: K's first, then V's
   uint4 codes[ST];
   uint32_t scales[ST];
-  auto fetch = [&](int kb) __attribute__((always_inline)) {
-    const Half H0 = half_at(kb, 0), H1 = half_at(kb, 1);
+  auto fetch = [&](Half H0, Half H1) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < ST; ++j) {
       const int n = j * 64 * NW + threadIdx.x, r = n / (HD / 32) % kPT, b = n % (HD / 32);
@@ -192,16 +223,25 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int p = 4 * b + k;
-        row[isv ? v_piece<HD>(r, p) : k_piece<HD>(r, p)] = __builtin_bit_cast(uint4, q4_frag(w[k], d2));
+        row[piece(r & 15, p)] = __builtin_bit_cast(uint4, q4_frag(w[k], d2));
       }
     }
   };
 
+  if (threadIdx.x == 0) *mark = 0;  // (a barrier comes before its first use)
+  uint32_t entry[2];  // of the tile behind the one that is staged
+  uint32_t there = 0, there_next = 0;
   if (n_tiles > 0) {
-    if constexpr (Q4)
-      fetch(R.base(first));
-    else
-      copy(bufs[0], R.base(first));
+    ask(0, entry);
+    const Half H0 = half_of(R.base(first), 0, entry[0]), H1 = second_half(H0, R.base(first), entry[1]);
+    there_next = (H0.there ? 1u : 0u) | (H1.there ? 2u : 0u);
+    if constexpr (Q4) {
+      fetch(H0, H1);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) copy(buf_of(0), H0, H1, n);
+    }
+    ask(1, entry);
   }
   // Q^T: dims 32 k + 8 g4 .. + 7
   h8v q[F][QS];
@@ -214,13 +254,15 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
       const int64_t a = q_at + k * 32 + g4 * 8;
       if constexpr (Q16) {
         q[f][k] = *reinterpret_cast<const h8v*>((const uint16_t*)A.q + a);
+        if (A.scale < 0.f) q[f][k] = -q[f][k];
       } else {
-        const float4 x = *reinterpret_cast<const float4*>((const float*)A.q + a);
-        const float4 y = *reinterpret_cast<const float4*>((const float*)A.q + a + 4);
-        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        const float4 v0 = *reinterpret_cast<const float4*>((const float*)A.q + a);
+        const float4 v1 = *reinterpret_cast<const float4*>((const float*)A.q + a + 4);
+        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          const _Float16 hi = (_Float16)v[t], lo = (_Float16)(v[t] - (float)hi);
+          const float x = A.scale < 0.f ? -v[t] : v[t];
+          const _Float16 hi = (_Float16)x, lo = (_Float16)(x - (float)hi);
           q[f][k][t] = c < 8 ? hi : lo;
         }
       }
@@ -235,32 +277,44 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[f][d] = f4v{0.f, 0.f, 0.f, 0.f};
   }
-  const float scale2 = A.scale * 1.44269504088896341f;
+  // scores are taken in powers of 2; the sign of a negative scale is the
+  // queries', and a scale of 0 is next to it (a masked score times it is -inf)
+  const float scale2 = fmaxf(fabsf(A.scale) * 1.44269504088896341f, 1e-37f);
   // Byte offsets in a tile of this lane's part of K row c, dims 8 g4, and of V
   // row 4 g4 + c / 4, dims 4 (c % 4); other dims are an xor away.  Kept from the
   // compiler's view in the loop: the 24 sums would be held in registers.
   const int vrow = 4 * g4 + (c >> 2);
-  int kx = k_piece<HD>(c, g4) * 16, vx = v_piece<HD>(vrow, (c & 3) >> 1) * 16 + (c & 1) * 8;
+  int kx = (c * KP + piece(c, g4)) * 16, vx = (vrow * KP + piece(vrow, (c & 3) >> 1)) * 16 + (c & 1) * 8;
 
   // scores of this wave's columns with the keys of a tile
-  auto scores = [&](const uint4* buf, f4v(&sc)[F][2]) __attribute__((always_inline)) {
+  // (`beside`: what else is issued in its steps, one call a step)
+  auto scores = [&](const uint4* buf, uint4* ahead, f4v(&sc)[F][2], auto beside) __attribute__((always_inline)) {
 #pragma unroll
     for (int f = 0; f < F; ++f) sc[f][0] = sc[f][1] = f4v{0.f, 0.f, 0.f, 0.f};
+    h8v ka[kAhead + 1];  // fragments in flight: step k, half u is number 2 k + u
+    auto ld_k = [&](int n) __attribute__((always_inline)) {
+      ka[n % (kAhead + 1)] = *reinterpret_cast<const h8v*>(
+          reinterpret_cast<const char*>(buf + 16 * (n & 1) * KP) + (kx ^ (64 * (n >> 1))));
+    };
 #pragma unroll
-    for (int k = 0; k < QS; ++k)
+    for (int n = 0; n < kAhead; ++n) ld_k(n);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const h8v ka = *reinterpret_cast<const h8v*>(reinterpret_cast<const char*>(buf + (16 * u + c) * KP) + (kx ^ (64 * k)));
+    for (int n = 0; n < 2 * QS; ++n) {
+      if (n + kAhead < 2 * QS) ld_k(n + kAhead);
+      if (n & 1) beside(ahead, n >> 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int f = 0; f < F; ++f) sc[f][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[f][k], sc[f][u], 0, 0, 0);
-      }
+      for (int f = 0; f < F; ++f)
+        sc[f][n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[n % (kAhead + 1)], q[f][n >> 1], sc[f][n & 1], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int f = 0; f < F; ++f)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float x = sc[f][j >> 2][j & 3];
         if constexpr (!Q16) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
-        sc[f][j >> 2][j & 3] = x * scale2;
+        sc[f][j >> 2][j & 3] = x;
       }
   };
   auto mask_scores = [&](int kb, uint32_t there, f4v(&sc)[F][2]) __attribute__((always_inline)) {
@@ -289,20 +343,23 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       x[u] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr4*)(
-                                         reinterpret_cast<const char*>(buf + TP + (16 * u + vrow) * KP) + (vx ^ (32 * d)))));
+                                         reinterpret_cast<const char*>(buf + TP + 16 * u * KP) + (vx ^ (32 * d)))));
     return __builtin_bit_cast(h8v, make_uint4(x[0].x, x[0].y, x[1].x, x[1].y));
   };
-  auto tile = [&](const uint4* buf, int kb, bool whole, uint32_t there) __attribute__((always_inline)) {
+  auto tile = [&](const uint4* buf, uint4* ahead, int kb, bool whole, uint32_t there, auto beside) __attribute__((always_inline)) {
     f4v sc[F][2];
-    scores(buf, sc);
+    scores(buf, ahead, sc, beside);
     if (!whole) mask_scores(kb, there, sc);
+    h8v vf[kAheadV + 1];
+#pragma unroll
+    for (int d = 0; d < kAheadV; ++d) vf[d] = ld_v(buf, d);
     h8v pf[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       float top = kNone;
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = fmaxf(top, sc[f][j >> 2][j & 3]);
-      top = quad_max4(top);
+      top = quad_max4(top) * scale2;
       if (__any(top > m[f] + 8.f)) {
         const float mn = fmaxf(m[f], top), a = exp2_(m[f] - mn);
         m[f] = mn;
@@ -312,16 +369,19 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float e = exp2_(sc[f][j >> 2][j & 3] - m[f]);
+        const float e = exp2_(fmaf(sc[f][j >> 2][j & 3], scale2, -m[f]));
         l[f] += e;
         weight(f, j, e, pf[f]);
       }
     }
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      const h8v v = ld_v(buf, d);
+      if (d + kAheadV < DT) vf[(d + kAheadV) % (kAheadV + 1)] = ld_v(buf, d + kAheadV);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int f = 0; f < F; ++f) o[f][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[f], o[f][d], 0, 0, 0);
+      for (int f = 0; f < F; ++f)
+        o[f][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d % (kAheadV + 1)], pf[f], o[f][d], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -332,7 +392,7 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
   // A row of V that a query does not see must not reach its output even as
   // 0 x infinity.  In a tile that some query does not see all of, rows that none
   // of them sees become zeros; true where another one holds a value that is not
-  // finite.  The whole workgroup calls it.
+  // finite, in this tile or one before.  The whole workgroup calls it.
   auto clean = [&](uint4* buf, int kb, uint32_t there) {
     bool found = false;
     for (int j = threadIdx.x; j < TP; j += 64 * NW) {
@@ -345,29 +405,58 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
       else
         found = found || not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
     }
-    return __syncthreads_or(found) != 0;
+    if (found) *mark = 1;
+    lds_sync();
+    return uni(*mark) != 0;
   };
   bool odd = false;
   for (int n = 0; n < n_tiles; ++n) {
     const int kb = R.base(first + n);
-    uint4* buf = bufs[n & 1];
+    uint4* buf = buf_of(n);
     asm volatile("" : "+v"(kx), "+v"(vx));
+    there = there_next;
+    const bool more = n + 1 < n_tiles;
+    const int kb1 = R.base(first + n + (more ? 1 : 0));
     if constexpr (Q4) {
       unpack(buf);
-      if (n + 1 < n_tiles) fetch(R.base(first + n + 1));
-      lds_sync();
     } else {
       // every wave's copies of this tile have landed, and every wave is done
       // with the buffer that the next ones overwrite
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
       lds_sync();
-      if (n + 1 < n_tiles) copy(bufs[(n + 1) & 1], R.base(first + n + 1));
+    }
+    const Half H0 = half_of(kb1, 0, entry[0]), H1 = second_half(H0, kb1, entry[1]);
+    there_next = (H0.there ? 1u : 0u) | (H1.there ? 2u : 0u);
+    if constexpr (Q4) {
+      if (more) {
+        fetch(H0, H1);
+        ask(n + 2, entry);
+      }
+      lds_sync();
     }
     // what the workgroup's rows, and what this wave's, see of it
-    const uint32_t there = (half_at(kb, 0).there ? 1u : 0u) | (half_at(kb, 1).there ? 2u : 0u);
-    if (!all_see(kb, there, pa, pb)) odd = clean(buf, kb, there) || odd;
+    if (!all_see(kb, there, pa, pb)) odd = clean(buf, kb, there);
     const bool past = kb > wp1, before = A.window > 0 && kb + kPT - 1 <= wp0 - A.window && kb >= A.sinks;
-    if (any && !past && !before) tile(buf, kb, all_see(kb, there, wp0, wp1), there);
+    // the next tile's copies go out between the products (one behind the other
+    // they hold up the wave for 500 clocks); the last tile's are its own again
+    auto beside = [&](uint4* ahead, int k) __attribute__((always_inline)) {
+      if constexpr (!Q4) {
+#pragma unroll
+        for (int j = k * NC / QS; j < (k + 1) * NC / QS; ++j) copy(ahead, H0, H1, j);
+        if (k == QS - 1) ask(n + 2, entry);
+      }
+    };
+    // (no alias between the two buffers: a copy into one needs no wait before the reads of the other)
+    auto step = [&](const uint4* __restrict__ cur, uint4* __restrict__ ahead) __attribute__((always_inline)) {
+      int sees = uni(any && !past && !before);
+      if (!sees) {
+#pragma unroll
+        for (int k = 0; k < QS; ++k) beside(ahead, k);
+      }
+      asm volatile("" : "+v"(sees));  // (joined with the branch above, it keeps two copies of the outputs)
+      if (uni(sees)) tile(cur, ahead, kb, all_see(kb, there, wp0, wp1), there, beside);
+    };
+    step(buf, buf_of(n + 1));
   }
   if (odd) {
     // (a broken cache) Row by row and key by key, a wave a row, from memory
@@ -383,12 +472,12 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
       }
       for (int n = 0; n < n_tiles; ++n)
         for (int key = R.base(first + n), end = key + kPT; key < end; ++key) {
-          const Half H = half_at(key & ~15, 0);
+          const Half H = half_of(key & ~15, 0, tab[min(key >> P.page_shift, P.table_stride - 1)]);
           if (!H.there || key >= cap || !key_seen(key, pos, A.window, A.sinks)) continue;
           float sc = 0.f;
 #pragma unroll
           for (int e = 0; e < E; ++e) sc = fmaf(x[e], cache_value<HD, Q4>(H.k, H.row + (key & 15), E * lane + e, P.page_shift), sc);
-          sc = wave_sum(sc) * scale2;
+          sc = wave_sum(sc) * A.scale * 1.44269504088896341f;
           const float mn = fmaxf(m1, sc), f = exp2_(m1 - mn), w = exp2_(sc - mn);
           m1 = mn;
           l1 = l1 * f + w;
@@ -480,7 +569,7 @@ int tile_rows(int hd, bool q16) {
   return hd == 512 ? (q16 ? kTileRows<512, true> : kTileRows<512, false>)
                    : (q16 ? kTileRows<256, true> : kTileRows<256, false>);
 }
-// at most this many tiles: each sequence's last may be part full
+// at most this many tiles (each sequence's last may be part full)
 int64_t tile_bound(const PagedAttnArgs& a, int bm) {
   return (int64_t)a.P.n_tok * a.gqa / bm + std::min(a.P.n_seq, a.P.n_tok);
 }
@@ -504,10 +593,12 @@ int chunk_hd(const PagedAttnArgs& a, bool q4, hipStream_t st) {
 
 void plan_attn_paged_chunk(PagedAttnArgs& a, int hd, bool q16) {
   const int bm = tile_rows(hd, q16);
-  const int64_t units = tile_bound(a, bm) * a.P.kvh;
+  const int64_t units = tile_bound(a, bm) * a.P.kvh;  // the grid's; `full`: about as many have work
+  const int64_t full = std::max<int64_t>(1, ((int64_t)a.P.n_tok * a.gqa + bm - 1) / bm) * a.P.kvh;
   const int64_t seen = a.window ? std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + bm / a.gqa + 1) : a.max_kv;
   const int64_t tiles = seen / kPT + 2;
-  int64_t ns = std::min<int64_t>((512 + units - 1) / units, tiles / kMinTiles);
+  // two workgroups fill a CU
+  const int64_t ns = std::min<int64_t>(2 * 256 / full, tiles / kMinTiles);
   a.ns = (int)std::max<int64_t>(1, std::min<int64_t>(ns, 64));
   a.part_floats = a.ns > 1 ? (size_t)units * a.ns * bm * hd : 0;
   a.ml_floats = a.ns > 1 ? (size_t)units * a.ns * bm * 2 : 0;
