@@ -33,8 +33,11 @@ int check_call(const char* fn, const e4b_paged_kv* kv, const e4b_kv_batch* b, Pa
   int rc = check_cache(fn, kv);
   if (rc) return rc;
   if (!b) return e4b_fail(E4B_EINVAL, "%s: null batch", fn);
-  if (b->n_seq < 0 || b->n_tok < 0 || b->n_seq > 65535 || b->n_tok > (1 << 24))
-    return e4b_fail(E4B_EINVAL, "%s: %d sequences (0 .. 65535), %d tokens (0 .. 2^24)", fn, b->n_seq, b->n_tok);
+  // (a grid's threads are below 2^32: tokens by 256, units of attention by 512)
+  if (b->n_seq < 0 || b->n_tok < 0 || b->n_seq > 65535 || b->n_tok >= (1 << 24) ||
+      (int64_t)b->n_seq * kv->kv_heads > (1 << 21))
+    return e4b_fail(E4B_EINVAL, "%s: %d sequences (0 .. 65535, %d KV heads: 2^21 of both), %d tokens (below 2^24)", fn,
+                    b->n_seq, kv->kv_heads, b->n_tok);
   *empty = b->n_seq == 0 || b->n_tok == 0;
   if (*empty) return E4B_OK;
   if (!b->q_start || !b->kv_len || !aligned(b->q_start, 4) || !aligned(b->kv_len, 4))
@@ -160,8 +163,8 @@ static int attn_setup(const char* fn, const e4b_paged_kv* kv, const e4b_kv_batch
     return e4b_fail(E4B_EINVAL, "%s: q dtype %d (E4B_DT_F32 or E4B_DT_F16)", fn, q_dtype);
   if (window < 0 || sinks < 0) return e4b_fail(E4B_EINVAL, "%s: window %d, sinks %d", fn, window, sinks);
   if (*empty) return E4B_OK;
-  if ((int64_t)batch->n_tok * q_heads > (1 << 30))
-    return e4b_fail(E4B_EINVAL, "%s: %d tokens of %d heads are more than 2^30 rows", fn, batch->n_tok, q_heads);
+  if ((int64_t)batch->n_tok * q_heads > (1 << 28))
+    return e4b_fail(E4B_EINVAL, "%s: %d tokens of %d heads are more than 2^28 rows", fn, batch->n_tok, q_heads);
   a.qh = q_heads;
   a.gqa = q_heads / kv->kv_heads;
   a.window = window;

@@ -323,8 +323,8 @@ typedef struct e4b_paged_kv {
 typedef struct e4b_kv_batch {
   const int32_t* q_start; /* [n_seq + 1], not falling; q_start[0] = 0 unless tokens before are to be skipped */
   const int32_t* kv_len;  /* [n_seq] */
-  int32_t n_seq;          /* <= 65535 */
-  int32_t n_tok;          /* token rows of the buffers, >= q_start[n_seq], <= 2^24 */
+  int32_t n_seq;          /* <= 65535, and n_seq * kv_heads <= 2^21 */
+  int32_t n_tok;          /* token rows of the buffers, >= q_start[n_seq], < 2^24 */
   int32_t max_q;
   int32_t max_kv;
 } e4b_kv_batch;
@@ -376,8 +376,10 @@ int e4b_attn_paged_ws_bytes(const e4b_paged_kv* kv, const e4b_kv_batch* batch, i
  *   out[t][h] = sum_k softmax_k(scale q.k) v_k   (f16, rows out_stride apart)
  * over the keys k <= p of the token's position p with k > p - window or
  * k < sinks (window 0: all of them); KV head h / (q_heads / kv_heads).  A
- * token that sees no key gets zeros.  What masked, absent or unused rows hold
- * does not matter, infinities and NaN included.
+ * token that sees no key, or whose scores are all -infinity, gets zeros.  What
+ * masked, absent or unused rows hold does not matter, infinities and NaN
+ * included.  f32 queries are used to 2^-22 of their value and must be below
+ * 65520 in magnitude; at most 2^28 rows (n_tok * q_heads).
  * ws: scratch of e4b_attn_paged_ws_bytes bytes, 16-byte aligned, for this call
  * alone until it has run; NULL: the library's workspace (calls on one device
  * that use it must be ordered; see "Workspace" above). */

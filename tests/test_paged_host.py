@@ -176,3 +176,41 @@ def test_reference_codes():
     assert np.mean(np.abs(v - x) <= step * 0.5 * (1 + 2.0**-4)) > 0.97
     b = x.reshape(40, 8, 32)
     assert np.all(np.take_along_axis(codes.reshape(40, 8, 32), np.abs(b).argmax(-1)[..., None], -1) == 0)
+
+
+@pytest.mark.parametrize("call", [append, gather, attn], ids=["append", "gather", "attn"])
+def test_batches_past_the_grids(call):
+    """A grid holds fewer than 2^32 threads."""
+    assert call(b=batch(n_tok=1 << 24)) == E4B_EINVAL and "2^24" in _lib.last_error()
+    for n_seq, kvh in ((65535, 33), (8193, 256)):
+        kw = {} if call is not attn else dict(qh=kvh, qs=kvh * 256, os=kvh * 256)
+        assert call(kv=cache(kv_heads=kvh), b=batch(n_seq=n_seq), **kw) == E4B_EINVAL
+        assert "2^21" in _lib.last_error()
+
+
+def test_rows_past_the_grid_of_attention():
+    qh = 4096
+    for n_tok, rc in ((1 << 16, E4B_OK), ((1 << 16) + 1, E4B_EINVAL)):
+        n = C.c_size_t(0)
+        assert lib.e4b_attn_paged_ws_bytes(C.byref(cache()), C.byref(batch(n_tok=n_tok)), DT_F32, qh, 0, 0,
+                                           C.byref(n)) == rc
+    assert "2^28" in _lib.last_error()
+
+
+def test_scratch_that_is_too_small_or_not_aligned():
+    n = C.c_size_t(0)
+    b = batch(n_seq=1, n_tok=1, max_q=1, max_kv=4000)
+    assert lib.e4b_attn_paged_ws_bytes(C.byref(cache()), C.byref(b), DT_F32, 8, 0, 0, C.byref(n)) == E4B_OK
+    assert n.value > 0
+    for ws, size in ((P, n.value - 1), (P, 0), (P + 8, n.value)):
+        assert attn(b=b, ws=ws, wb=size) == E4B_EINVAL
+        assert "scratch" in _lib.last_error()
+
+
+def test_scratch_does_not_depend_on_pointers():
+    sizes = []
+    for over in ({}, dict(q_start=P + 4, kv_len=P + 8)):
+        bb, n = batch(n_seq=3, n_tok=900, max_q=400, max_kv=9000, **over), C.c_size_t(0)
+        assert lib.e4b_attn_paged_ws_bytes(C.byref(cache()), C.byref(bb), DT_F16, 8, 0, 0, C.byref(n)) == E4B_OK
+        sizes.append(n.value)
+    assert sizes[0] == sizes[1]
