@@ -126,7 +126,8 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
   const int rows = s.n * A.gqa;
   const int t0 = qt * BM, t1 = min(t0 + BM, rows);  // rows of the tile
   const int cap = paged_cap(P);
-  const int pa = s.p0 + uni(t0 / A.gqa), pb = s.p0 + uni((t1 - 1) / A.gqa);  // their positions
+  // their positions (the first that there can be: a window is taken off it)
+  const int pa = max(0, s.p0 + uni(t0 / A.gqa)), pb = s.p0 + uni((t1 - 1) / A.gqa);
   const TileRange R = tile_range(pa, pb, A.window, A.sinks, cap);
   const int per = chunk_per(R.n, A.ns), live = uni((R.n + per - 1) / per);  // tiles of a split, splits that have any
   const int n_tiles = max(0, min(per, R.n - sp * per)), first = sp * per;
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
   // this wave's rows, and this lane's column of each fragment
   const int w0 = t0 + wave * F * RF, w1 = min(w0 + F * RF, t1);
   const bool any = w0 < t1;
-  const int wp0 = s.p0 + uni(min(w0, rows - 1) / A.gqa), wp1 = s.p0 + uni((max(w1, 1) - 1) / A.gqa);
+  const int wp0 = max(0, s.p0 + uni(min(w0, rows - 1) / A.gqa)), wp1 = s.p0 + uni((max(w1, 1) - 1) / A.gqa);
   int tok[F];
 #pragma unroll
   for (int f = 0; f < F; ++f) tok[f] = min(w0 + f * RF + (c & (RF - 1)), rows - 1) / A.gqa;

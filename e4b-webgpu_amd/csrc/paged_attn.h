@@ -33,11 +33,11 @@ struct TileRange {
   DEV int base(int t) const { return (t < sink ? t : t - sink + from) * kPT; }
 };
 DEV TileRange tile_range(int p0, int p1, int window, int sinks, int cap) {
-  const int first = window > 0 ? max(0, p0 - window + 1) : 0;
+  const int first = window > 0 ? max(0, max(0, p0) - window + 1) : 0;  // (p0 < 0: no key, and any window may be taken off 0)
   const int last = min(p1, cap - 1);
   TileRange r;
   r.from = first / kPT;
-  r.sink = min((min(sinks, first) + kPT - 1) / kPT, r.from);
+  r.sink = min((int)(((uint32_t)min(sinks, first) + kPT - 1) / kPT), r.from);
   r.n = last < 0 ? 0 : min(r.sink, last / kPT + 1) + max(0, last / kPT - r.from + 1);
   return r;
 }

@@ -275,3 +275,16 @@ def test_ragged_batches_whose_splits_are_dealt_out(kind, n_seq, kv, q):
     rig.host.table[:, :kv // 64 + 1] = rng.integers(0, 50, (n_seq, kv // 64 + 1))
     rig.push()
     check_attn(rig, [q] * n_seq, kv_len, queries(rng, q * n_seq, 4, 128, DT_F32), 4, DT_F32, scale=0.09)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q4"])
+@pytest.mark.parametrize("window,sinks", [(2**31 - 1, 0), (2**31 - 1, 2**31 - 1), (3, 2**31 - 1)])
+def test_the_widest_windows_with_more_new_tokens_than_kept(kind, window, sinks):
+    rng = np.random.default_rng(82)
+    q_len, kv_len = [4, 40, 1, 90], [1, 9, 30, 70]
+    rig = Rig(kind, 128, 2, 16, 4, 80)
+    rig.host.fill(rng, kv_len)
+    rig.push()
+    for qt in (DT_F32, DT_F16):
+        check_attn(rig, q_len, kv_len, queries(rng, sum(q_len), 8, 128, qt), 8, qt, window, sinks, scale=0.09)
+        check_attn(rig, q_len[:1], kv_len[:1], queries(rng, 4, 8, 128, qt), 8, qt, window, sinks, scale=0.09)
