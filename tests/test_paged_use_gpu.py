@@ -288,3 +288,35 @@ def test_the_widest_windows_with_more_new_tokens_than_kept(kind, window, sinks):
     for qt in (DT_F32, DT_F16):
         check_attn(rig, q_len, kv_len, queries(rng, sum(q_len), 8, 128, qt), 8, qt, window, sinks, scale=0.09)
         check_attn(rig, q_len[:1], kv_len[:1], queries(rng, 4, 8, 128, qt), 8, qt, window, sinks, scale=0.09)
+
+
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 128, 4096, 4097, 9000])
+def test_append_to_many_sequences(n):
+    """Every token finds its sequence, with empty ones among them and tokens before the first and behind the last."""
+    rng = np.random.default_rng(n)
+    hd, skip, behind = 128, 3, 5
+    q_len = rng.integers(0, 3, n)
+    q_len[rng.integers(n)] = 6
+    kv_len = (q_len + rng.integers(0, 10, n)).astype(np.int32)
+    start = (skip + np.concatenate([[0], np.cumsum(q_len)])).astype(np.int32)
+    n_tok = int(start[-1]) + behind
+    table = rng.permutation(n).astype(np.uint32)
+    kv = PagedKV("f16", 1, hd, 16, n, 1, table=DeviceBuffer.from_array(table))
+    kv.k.fill(0xFF)
+    kv.v.fill(0xFF)
+    x = rng.standard_normal((n_tok, 2, hd)).astype(np.float32)
+    b = KvBatch(DeviceBuffer.from_array(start), DeviceBuffer.from_array(kv_len), n, n_tok, 6, 16)
+    kv.append_dev(b, HeadPrep(None, None, None, 0, EPS, v_rms=False), DeviceBuffer.from_array(x), DT_F32, 0)
+    want = np.full((2, n, 16, hd), 0xFFFF, np.uint16)
+    for i in range(n):
+        for j in range(q_len[i]):
+            want[:, table[i], kv_len[i] - q_len[i] + j] = x[start[i] + j].astype(np.float16).view(np.uint16)
+    np.testing.assert_array_equal(kv.k.download(np.uint16).reshape(n, 16, hd), want[0])
+    np.testing.assert_array_equal(kv.v.download(np.uint16).reshape(n, 16, hd), want[1])
+    ko, vo = (DeviceBuffer.from_array(np.full((n_tok, hd), MARK, np.uint16)) for _ in "kv")
+    kv.gather_dev(b, ko, vo)
+    for j, o in enumerate((ko, vo)):
+        got = o.download(np.uint16).reshape(n_tok, hd)
+        assert (got[:skip] == MARK).all() and (got[n_tok - behind:] == MARK).all()
+        np.testing.assert_array_equal(got[skip:n_tok - behind],
+                                      x[skip:n_tok - behind, j].astype(np.float16).view(np.uint16))
