@@ -30,16 +30,13 @@
 namespace {
 
 constexpr int kRows = 8;
-constexpr int kWaves = 8;
 // Waves that share a tile.  Head dim 512 has no room for all of the output
 // (128 registers) beside the rows in flight: two waves take half of the dims
 // each, add up their halves of the scores through LDS, and keep half of V's.
 template <int HD>
 constexpr int kParts = HD / 256 > 1 ? 2 : 1;
-template <int HD>
-constexpr int kStreams = kWaves / kParts<HD>;  // tiles at a time in a workgroup
 
-// Splits.  A workgroup fills a CU, so there are about as many as CUs (one
+// Splits.  A workgroup of 8 waves fills a CU, so there are about as many as CUs (one
 // token at 32767 positions in 4 bits 15.7 us with 256 workgroups, 21.2 with
 // 512), dealt out by the sequences' lengths.  A split is a launch more (about
 // 4 us), and what it saves is the time in which one CU takes in its share: none
@@ -75,8 +72,9 @@ struct Slot {
 // Without splits workgroup and unit are the same.  Else a unit has a split for
 // each `per` tiles (and takes even shares of its tiles), per being as small as
 // leaves no more than A.groups workgroups in all, from the lengths of all
-// sequences (a lane a sequence, 64 at a time; 131072 units at most).  The slot of workgroup `at`, or (by
-// unit) of the unit `at` with sp = 0; seq < 0: there is none.
+// sequences (a lane a sequence, 64 at a time; 131072 units at most).  The slot
+// of workgroup `at`, or (by unit) of the unit `at` with sp = 0; seq < 0: there
+// is none.
 DEV int quotient(int a, int b) {  // a / b for a < 2^21: the error of (a + 1/2) / b in f32 is below 1 / (2 b)
   return uni((int)(((float)a + 0.5f) / (float)b));
 }
@@ -209,9 +207,9 @@ DEV void ld_dwords(const uint8_t* p, uint32_t* x) {
   }
 }
 
-template <int HD, bool Q4, bool Q16>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs A) {
-  constexpr int W = kStreams<HD>, VP = kParts<HD>, HW = HD / VP, NH = HW / 128, QS = HW / 32;  // HW: dims of a wave
+template <int HD, bool Q4, bool Q16, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_few(PagedAttnArgs A) {
+  constexpr int VP = kParts<HD>, W = NW / VP, HW = HD / VP, NH = HW / 128, QS = HW / 32;  // HW: dims of a wave
   constexpr int LD = HD + 4;  // floats between rows in LDS
   extern __shared__ __align__(16) float lds[];  // queries; later [W][rows][LD] outputs, [W][8][2] maxima and sums
   const PagedArgs& P = A.P;
@@ -311,12 +309,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   // registers they would cost every wave HD / 8 of them.  Their loads go out
   // first, then the first tile's.
   h8v* qf = reinterpret_cast<h8v*>(lds);
-  constexpr int QF = HD / 32, QN = (QF + kWaves - 1) / kWaves;  // fragments, and of a wave
+  constexpr int QF = HD / 32, QN = (QF + NW - 1) / NW;  // fragments, and of a wave
   uint32_t qraw[QN][Q16 ? 4 : 8];
   const int64_t q_at = (int64_t)(s.q0 + ro.tok) * A.q_stride + ro.head * HD;
 #pragma unroll
   for (int j = 0; j < QN; ++j) {
-    const int f = min(j * kWaves + wave, QF - 1), k = f % QS, d = f / QS * HW + (Q4 ? (g4 * QS + k) * 8 : k * 32 + g4 * 8);
+    const int f = min(j * NW + wave, QF - 1), k = f % QS, d = f / QS * HW + (Q4 ? (g4 * QS + k) * 8 : k * 32 + g4 * 8);
     const uint8_t* p = (const uint8_t*)A.q + (q_at + d) * (Q16 ? 2 : 4);
     ld_dwords<4>(p, qraw[j]);
     if constexpr (!Q16) ld_dwords<4>(p + 16, qraw[j] + 4);
@@ -333,7 +331,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int j = 0; j < QN; ++j) {
-    const int k = j * kWaves + wave;
+    const int k = j * NW + wave;
     h8v q;
     if constexpr (Q16) {
       q = __builtin_bit_cast(h8v, make_uint4(qraw[j][0], qraw[j][1], qraw[j][2], qraw[j][3]));
@@ -394,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
     scores(0);
     scores(1);
     if constexpr (VP == 2) {
-      f4v* xs = reinterpret_cast<f4v*>(lds + HD * 8) + round * (kWaves * 128);
+      f4v* xs = reinterpret_cast<f4v*>(lds + HD * 8) + round * (NW * 128);
 #pragma unroll
       for (int u = 0; u < 2; ++u) xs[wave * 128 + u * 64 + lane] = sc[u];
       lds_sync();
@@ -543,7 +541,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_attn_paged_few(PagedAttnArgs
     }
   if (part == 0 && lane < rows) *reinterpret_cast<float2*>(ml + (stream * kRows + lane) * 2) = make_float2(m, l);
   lds_sync();
-  for (int e = threadIdx.x; e < rows * (HD / 4); e += 64 * kWaves) {
+  for (int e = threadIdx.x; e < rows * (HD / 4); e += 64 * NW) {
     const int r = e / (HD / 4), d = e % (HD / 4) * 4;
     float2 st[W];
     float M = kNone, L = 0.f;
@@ -640,24 +638,35 @@ __global__ __launch_bounds__(256) void k_attn_paged_merge(PagedAttnArgs A) {
   }
 }
 
-template <int HD>
-int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
-  constexpr int W = kStreams<HD>;
-  const int nr = std::min(a.max_q * a.gqa, kRows), units = a.P.n_seq * a.P.kvh * a.nrb;
-  const size_t lds = std::max((size_t)W * nr * (HD + 4) * 4 + W * kRows * 8, (size_t)HD * 32 + (kParts<HD> == 2 ? 2 * kWaves * 128 * 16 : 0));
+template <int HD, int NW>
+int few_waves(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
+  constexpr int W = NW / kParts<HD>;
+  const int nr = std::min(a.max_q * a.gqa, kRows);
+  const size_t lds = std::max((size_t)W * nr * (HD + 4) * 4 + W * kRows * 8, (size_t)HD * 32 + (kParts<HD> == 2 ? 2 * NW * 128 * 16 : 0));
   const dim3 grid((unsigned)a.groups);
   auto go = [&](auto* kernel) {
     // (more than 64 KB of LDS has to be asked for; 67 KB at most here)
     if (lds > 65536)
       E4B_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    kernel<<<grid, 64 * kWaves, lds, st>>>(a);
+    kernel<<<grid, 64 * NW, lds, st>>>(a);
     E4B_HIP(hipGetLastError());
     return E4B_OK;
   };
-  int rc = q4 && q16 ? go(k_attn_paged_few<HD, true, true>)
-           : q4      ? go(k_attn_paged_few<HD, true, false>)
-           : q16     ? go(k_attn_paged_few<HD, false, true>)
-                     : go(k_attn_paged_few<HD, false, false>);
+  return q4 && q16 ? go(k_attn_paged_few<HD, true, true, NW>)
+         : q4      ? go(k_attn_paged_few<HD, true, false, NW>)
+         : q16     ? go(k_attn_paged_few<HD, false, true, NW>)
+                   : go(k_attn_paged_few<HD, false, false, NW>);
+}
+
+template <int HD>
+int few_hd(const PagedAttnArgs& a, bool q4, bool q16, hipStream_t st) {
+  const int nr = std::min(a.max_q * a.gqa, kRows), units = a.P.n_seq * a.P.kvh * a.nrb;
+  // Two units a CU or more: workgroups of 4 waves, two on a CU, one's first
+  // loads and merge beside the other's tiles (200 ragged sequences of up to 500
+  // positions, 8 KV heads of 128: f16 67 us with 8 waves, 53 with 4; 4 bits 49
+  // and 30).  Fewer units than that leave CUs with one workgroup (128 sequences
+  // of up to 2000 positions, 2 KV heads of 256, f16: 70 and 78).
+  const int rc = units >= 2 * kGroups ? few_waves<HD, 4>(a, q4, q16, st) : few_waves<HD, 8>(a, q4, q16, st);
   if (rc || !a.split) return rc;
   // a few rows: more workgroups a row, each with fewer splits to add up in turn
   if (units * nr < 128)

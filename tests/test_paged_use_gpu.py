@@ -320,3 +320,23 @@ def test_append_to_many_sequences(n):
         assert (got[:skip] == MARK).all() and (got[n_tok - behind:] == MARK).all()
         np.testing.assert_array_equal(got[skip:n_tok - behind],
                                       x[skip:n_tok - behind, j].astype(np.float16).view(np.uint16))
+
+
+@pytest.mark.parametrize("kind,hd,kvh,g", [("f16", 256, 8, 2), ("q4", 128, 16, 1), ("q4", 512, 4, 3), ("f16", 128, 256, 1),
+                                           ("f16", 512, 8, 8)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_batches_of_many_units(kind, hd, kvh, g, window):
+    """More (sequence, KV head)s than two a CU, with lengths of one token to several tiles for each wave."""
+    rng = np.random.default_rng(hd + kvh)
+    n = 1300 // kvh
+    rig = Rig(kind, hd, kvh, 32, 1, 16, n_pages=2)
+    base = ref.Cache(kind, kvh, hd, 32, 12, 1, 12)
+    base.fill(rng, [12 * 32])
+    base.table = rng.integers(0, 12, (n, 12)).astype(np.uint32)
+    base.stride = 12
+    rig.host, rig.dev = base, PagedKV(kind, kvh, hd, 32, 12, 12, n_seq=n)
+    rig.push()
+    kv_len = rng.integers(1, 380 if n < 100 else 130, n)
+    kv_len[0], kv_len[-1] = 1, 380
+    check_attn(rig, [1] * n, kv_len, queries(rng, n, kvh * g, hd, DT_F32), kvh * g, DT_F32, window, 5 if window else 0,
+               scale=hd**-0.5)
