@@ -49,30 +49,38 @@ constexpr int kTileRows = kChunkWaves<HD> * kFrags<HD> * (Q16 ? 16 : 8);
 // see the most keys.
 struct TileAt {
   int seq, tile;
+  SeqSpan s;
 };
 DEV TileAt find_tile(const PagedAttnArgs& A, int rows_per, int at) {
+  const PagedArgs& P = A.P;
   const int lane = threadIdx.x & 63;
-  for (int b = 0; b < A.P.n_seq; b += 64) {
-    int n = 0;
-    if (b + lane < A.P.n_seq) {
-      const int q0 = min(max(A.P.q_start[b + lane], 0), A.P.n_tok);
-      const int rows = (min(max(A.P.q_start[b + lane + 1], q0), A.P.n_tok) - q0) * A.gqa;
-      n = rows <= A.few_rows ? 0 : (rows + rows_per - 1) / rows_per;
-    }
+  for (int b = 0; b < P.n_seq; b += 64) {
+    const int i = min(b + lane, P.n_seq - 1);
+    const int start = P.q_start[i], end = P.q_start[i + 1], kv = P.kv_len[i];  // (all at once: each is a trip to memory)
+    const int rows = seq_span_of(P, start, end, kv).n * A.gqa;
+    const int n = b + lane >= P.n_seq || rows <= A.few_rows ? 0 : (rows + rows_per - 1) / rows_per;
     const int upto = wave_scan(n);
     const uint64_t past = __ballot(at < upto);
     if (past) {
       const int f = __builtin_ctzll(past);
-      const int last = __builtin_amdgcn_readlane(upto, f) - 1 - at;
-      return {b + f, last};
+      return {b + f, __builtin_amdgcn_readlane(upto, f) - 1 - at,
+              seq_span_of(P, __builtin_amdgcn_readlane(start, f), __builtin_amdgcn_readlane(end, f),
+                          __builtin_amdgcn_readlane(kv, f))};
     }
     at -= last_lane(upto);
   }
-  return {-1, 0};
+  return {-1, 0, {}};
 }
 
 constexpr int kMinTiles = 8;  // key tiles of a split at least
 DEV int chunk_per(int n, int ns) { return max(kMinTiles, uni((n + ns - 1) / ns)); }
+
+// what the wave's lanes wrote to LDS is there for all of them
+DEV void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // whether one of two f16 values is not finite
 DEV bool not_finite(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
@@ -122,7 +130,7 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
   const TileAt ta = find_tile(A, BM, at);
   const int i = __builtin_amdgcn_readfirstlane(ta.seq), qt = __builtin_amdgcn_readfirstlane(ta.tile);
   if (i < 0) return;
-  const SeqSpan s = seq_span(P, i);
+  const SeqSpan s = ta.s;
   const int rows = s.n * A.gqa;
   const int t0 = qt * BM, t1 = min(t0 + BM, rows);  // rows of the tile
   const int cap = paged_cap(P);
@@ -500,31 +508,60 @@ __global__ __launch_bounds__(64 * kChunkWaves<HD>, 2) void k_attn_paged_chunk(Pa
   }
 
   // ---- results ----
+  // A register's columns are 16 rows: stored from there, each store would touch
+  // 16 of them, 32 or 64 bytes each.  Through LDS (DC dims of a fragment in the
+  // wave's part of the tiles' buffers) whole rows are stored, 1 KB at a time.
+  constexpr int DC = HD < 256 ? HD : 256, RP = DC / 4;  // RP: 16-byte pieces of a row
+  static_assert(NW * 16 * RP == 4 * TP, "the waves' parts are the buffers");
+  if constexpr (!Q4) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the copies behind the last tile have landed
+  lds_sync();
+  f4v* mine = reinterpret_cast<f4v*>(lds) + wave * 16 * RP;
+  const bool direct = live <= 1;
 #pragma unroll
   for (int f = 0; f < F; ++f) {
     const float L = quad_sum4(l[f]);
     bool have;
     const int head = row_of(f, have);
-    uint16_t* out = A.out + (int64_t)(s.q0 + tok[f]) * A.out_stride + head * HD + 4 * g4;
-    const bool direct = live <= 1;
     const float inv = !direct ? 1.f : L == 0.f ? 0.f : 1.f / L;
-    const int64_t row = ((int64_t)(at * P.kvh + g) * A.ns + sp) * BM + (wave * F + f) * RF + (c & (RF - 1));
-    if (!direct && have && lane < RF) *reinterpret_cast<float2*>(A.part_ml + row * 2) = make_float2(m[f], L);
+    const int r0 = w0 + f * RF;  // rows of the fragment that there are: r0 .. r0 + n - 1
+    const int n = min(RF, t1 - r0);
+    const int64_t out_at = (int64_t)(s.q0 + tok[f]) * A.out_stride + head * HD;  // of this lane's column
+    const int64_t part_row = ((int64_t)(at * P.kvh + g) * A.ns + sp) * BM + r0 - t0;
+    if (!direct && have && lane < RF) *reinterpret_cast<float2*>(A.part_ml + (part_row + lane) * 2) = make_float2(m[f], L);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      float x[4];
+    for (int h = 0; h < HD / DC; ++h) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = o[f][d][r];
-        if constexpr (!Q16) x[r] += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x[r]), 0x128, 0xf, 0xf, true));
-        x[r] *= inv;
+      for (int d = 0; d < DC / 16; ++d) {
+        f4v x = o[f][h * (DC / 16) + d];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (!Q16) x[r] += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x[r]), 0x128, 0xf, 0xf, true));
+          x[r] *= inv;
+        }
+        if (c < RF) mine[c * RP + ((4 * d + g4) ^ c)] = x;
       }
-      if (!have || c >= RF) continue;
-      if (direct)
-        *reinterpret_cast<uint2*>(out + 16 * d) =
-            make_uint2((uint32_t)f2h(x[0]) | (uint32_t)f2h(x[1]) << 16, (uint32_t)f2h(x[2]) | (uint32_t)f2h(x[3]) << 16);
-      else
-        *reinterpret_cast<float4*>(A.part + row * HD + 16 * d + 4 * g4) = make_float4(x[0], x[1], x[2], x[3]);
+      wave_fence();
+      if (direct) {
+        constexpr int PL = RP / 2, RI2 = 64 / PL;  // lanes of a row (8 dims each), rows at a time
+#pragma unroll
+        for (int k = 0; k < RF; k += RI2) {
+          const int r = k + lane / PL, e = lane % PL;
+          const int64_t to = (int64_t)__shfl((int)(out_at >> 32), r, 64) << 32 | (uint32_t)__shfl((int)out_at, r, 64);
+          const f4v x = mine[r * RP + ((2 * e) ^ r)], y = mine[r * RP + ((2 * e + 1) ^ r)];
+          if (r < n)
+            *reinterpret_cast<uint4*>(A.out + to + h * DC + 8 * e) =
+                make_uint4((uint32_t)f2h(x[0]) | (uint32_t)f2h(x[1]) << 16, (uint32_t)f2h(x[2]) | (uint32_t)f2h(x[3]) << 16,
+                           (uint32_t)f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, (uint32_t)f2h(y[2]) | (uint32_t)f2h(y[3]) << 16);
+        }
+      } else {
+        constexpr int RI2 = 64 / RP;
+#pragma unroll
+        for (int k = 0; k < RF; k += RI2) {
+          const int r = k + lane / RP, e = lane % RP;
+          if (r < n) *reinterpret_cast<f4v*>(A.part + (part_row + r) * HD + h * DC + 4 * e) = mine[r * RP + (e ^ r)];
+        }
+      }
+      wave_fence();
     }
   }
 }
@@ -538,26 +575,54 @@ __global__ __launch_bounds__(256) void k_attn_chunk_merge(PagedAttnArgs A) {
   const TileAt ta = find_tile(A, BM, at);
   const int i = __builtin_amdgcn_readfirstlane(ta.seq), qt = __builtin_amdgcn_readfirstlane(ta.tile);
   if (i < 0) return;
-  const SeqSpan s = seq_span(P, i);
+  const SeqSpan s = ta.s;
   const int rows = s.n * A.gqa, t0 = qt * BM, t1 = min(t0 + BM, rows);
   const TileRange R = tile_range(s.p0 + t0 / A.gqa, s.p0 + (t1 - 1) / A.gqa, A.window, A.sinks, paged_cap(P));
   const int per = chunk_per(R.n, A.ns), live = uni((R.n + per - 1) / per);
   const int r = part * RW + threadIdx.x / T, d = threadIdx.x % T * 4;
   if (live <= 1 || t0 + r >= t1) return;
   const int64_t row = (int64_t)(at * P.kvh + g) * A.ns * BM + r;  // + sp * BM
+  // 4 splits at a time, the next ones' loads before these are added up
   float M = kNone, L = 0.f;
-  for (int sp = 0; sp < live; ++sp) M = fmaxf(M, A.part_ml[(row + (int64_t)sp * BM) * 2]);
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int sp = 0; sp < live; ++sp) {
-    const int64_t p = row + (int64_t)sp * BM;
-    const float2 st = *reinterpret_cast<const float2*>(A.part_ml + p * 2);
-    const float4 y = *reinterpret_cast<const float4*>(A.part + p * HD + d);
-    const float w = exp2_(st.x - M);
-    L += w * st.y;
-    x.x += w * y.x;
-    x.y += w * y.y;
-    x.z += w * y.z;
-    x.w += w * y.w;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y[4];
+  float2 st[4];
+  auto load = [&](int sp) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t p = row + (int64_t)min(sp + k, live - 1) * BM;
+      st[k] = *reinterpret_cast<const float2*>(A.part_ml + p * 2);
+      y[k] = *reinterpret_cast<const float4*>(A.part + p * HD + d);
+    }
+  };
+  load(0);
+  for (int sp = 0; sp < live; sp += 4) {
+    float2 s4[4];
+    float4 z[4];
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s4[k] = st[k];
+      z[k] = y[k];
+      top = fmaxf(top, st[k].x);  // (the last split again behind the last one)
+    }
+    if (sp + 4 < live) load(sp + 4);
+    const float a = exp2_(M - top);
+    M = top;
+    L *= a;
+    x.x *= a;
+    x.y *= a;
+    x.z *= a;
+    x.w *= a;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = sp + k < live ? exp2_(s4[k].x - M) : 0.f;
+      if (sp + k >= live) z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      L += w * (sp + k < live ? s4[k].y : 0.f);
+      x.x += w * z[k].x;
+      x.y += w * z[k].y;
+      x.z += w * z[k].z;
+      x.w += w * z[k].w;
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int rr = t0 + r, t = rr / A.gqa, h = g * A.gqa + rr % A.gqa;
