@@ -129,11 +129,14 @@ struct PagedAttnArgs {
   float* part;
   float* part_ml;
 };
-// a few query rows per sequence and KV head (k_paged_decode.hip)
+// a few query rows per sequence and KV head (paged_few.h)
 void plan_attn_paged_few(PagedAttnArgs& a, int hd);
 int launch_attn_paged_few(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
 constexpr int kPagedFewRows = 16;  // most rows of a sequence and KV head that it takes
-// any number (k_paged_chunk.hip)
+// any number (paged_chunk.h)
 void plan_attn_paged_chunk(PagedAttnArgs& a, int hd, bool q16);
 int launch_attn_paged_chunk(const PagedAttnArgs& a, int hd, bool q4, bool q16, hipStream_t st);
+// both (k_paged_mixed.hip)
+int launch_attn_paged_mixed(const PagedAttnArgs& chunk, const PagedAttnArgs& few, int hd, bool q4, bool q16,
+                            hipStream_t st);
 #endif

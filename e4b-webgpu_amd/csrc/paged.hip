@@ -231,9 +231,9 @@ extern "C" int e4b_k_attn_paged(const e4b_paged_kv* kv, const e4b_kv_batch* batc
     a->out_stride = out_stride;
     a->scale = scale;
     at = give_scratch(*a, at);
-    rc = a == &plan.chunk ? launch_attn_paged_chunk(*a, kv->head_dim, q4, q16, (hipStream_t)stream)
-                          : launch_attn_paged_few(*a, kv->head_dim, q4, q16, (hipStream_t)stream);
-    if (rc) return rc;
   }
-  return E4B_OK;
+  hipStream_t st = (hipStream_t)stream;
+  if (plan.use_chunk && plan.use_few) return launch_attn_paged_mixed(plan.chunk, plan.few, kv->head_dim, q4, q16, st);
+  return plan.use_chunk ? launch_attn_paged_chunk(plan.chunk, kv->head_dim, q4, q16, st)
+                        : launch_attn_paged_few(plan.few, kv->head_dim, q4, q16, st);
 }
