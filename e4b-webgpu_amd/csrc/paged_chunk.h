@@ -56,9 +56,17 @@ struct TileAt {
 DEV TileAt find_tile(const PagedAttnArgs& A, int rows_per, int at) {
   const PagedArgs& P = A.P;
   const int lane = threadIdx.x & 63;
-  for (int b = 0; b < P.n_seq; b += 64) {
+  int ahead[3];
+  auto load = [&](int b) {  // (all at once, and one round ahead: each is a trip to memory)
     const int i = min(b + lane, P.n_seq - 1);
-    const int start = P.q_start[i], end = P.q_start[i + 1], kv = P.kv_len[i];  // (all at once: each is a trip to memory)
+    ahead[0] = P.q_start[i];
+    ahead[1] = P.q_start[i + 1];
+    ahead[2] = P.kv_len[i];
+  };
+  load(0);
+  for (int b = 0; b < P.n_seq; b += 64) {
+    const int start = ahead[0], end = ahead[1], kv = ahead[2];
+    if (b + 64 < P.n_seq) load(b + 64);
     const int rows = seq_span_of(P, start, end, kv).n * A.gqa;
     const int n = b + lane >= P.n_seq || rows <= A.few_rows ? 0 : (rows + rows_per - 1) / rows_per;
     const int upto = wave_scan(n);
@@ -662,9 +670,11 @@ inline int tile_rows(int hd, bool q16) {
   return hd == 512 ? (q16 ? kTileRows<512, true> : kTileRows<512, false>)
                    : (q16 ? kTileRows<256, true> : kTileRows<256, false>);
 }
-// at most this many tiles (each sequence's last may be part full)
+// at most this many tiles: each sequence's last may be part full, and there
+// are no more sequences than rows allow
 inline int64_t tile_bound(const PagedAttnArgs& a, int bm) {
-  return (int64_t)a.P.n_tok * a.gqa / bm + std::min(a.P.n_seq, a.P.n_tok);
+  const int64_t rows = (int64_t)a.P.n_tok * a.gqa;
+  return rows / bm + std::min({(int64_t)a.P.n_seq, (int64_t)a.P.n_tok, rows / (a.few_rows + 1)});
 }
 // workgroups: of the attention, and of the merge (0: no split)
 template <int HD, bool Q16>

@@ -20,8 +20,11 @@
 //   takes V in the same key order.  A lane loads 8 keys' rows 4g + r, 8 dims
 //   of each, and turns them over in registers (one v_perm a pair): dims become
 //   rows of A without a pass through LDS.
-// What bounds it: the cache's bytes.  A tile of 32 keys is 32 KB (head dim
-// 256, f16) in flight per wave, a few microseconds of a CU's share of HBM.
+// What bounds it: in f16 the cache's bytes (64 tokens at 8192 positions, 2 KV
+// heads of 256: 1.07 GB in 186 us, 5.8 TB/s; a tile of 32 keys is 32 KB in
+// flight per wave); in 4 bits the unpacking (48 tokens at up to 4096, head dim
+// 512: 130 MB in 47 us, VALU 55 % of the issue slots); few tokens latency (one
+// at 300 positions 11.7 us).
 #pragma once
 #include <algorithm>
 
@@ -38,9 +41,9 @@ constexpr int kRows = 8;
 template <int HD>
 constexpr int kParts = HD / 256 > 1 ? 2 : 1;
 
-// Splits.  A workgroup of 8 waves fills a CU, so there are about as many as CUs (one
-// token at 32767 positions in 4 bits 15.7 us with 256 workgroups, 21.2 with
-// 512), dealt out by the sequences' lengths.  A split is a launch more (about
+// Splits.  A workgroup of 8 waves fills a CU, so there are about as many as CUs
+// (one token at 32767 positions in 4 bits 15.7 us with 256 workgroups, 21.2
+// with 512), dealt out by the sequences' lengths.  A split is a launch more (about
 // 4 us), and what it saves is the time in which one CU takes in its share: none
 // up to 7 tiles (one token at 128 positions 7.2 us in one workgroup, 9.0 in
 // two), shares of 4 tiles above (at 300 positions 10.6 us, 12.9 in one
