@@ -32,12 +32,27 @@ int chunk_hd(const PagedAttnArgs& a, bool q4, hipStream_t st) {
 
 void plan_attn_paged_chunk(PagedAttnArgs& a, int hd, bool q16) {
   const int bm = tile_rows(hd, q16);
-  const int64_t units = tile_bound(a, bm) * a.P.kvh;  // the grid's; `full`: about as many have work
-  const int64_t full = std::max<int64_t>(1, ((int64_t)a.P.n_tok * a.gqa + bm - 1) / bm) * a.P.kvh;
+  const int64_t units = tile_bound(a, bm) * a.P.kvh, rows = (int64_t)a.P.n_tok * a.gqa;  // units: the grid's
+  // Units that have work: known where all sequences are as long as the longest,
+  // else as if so many were and the others had a token each
+  const int64_t longest = std::min<int64_t>(
+      a.P.n_seq, std::max<int64_t>(1, (a.P.n_tok - a.P.n_seq + a.max_q - 2) / std::max(1, a.max_q - 1)));
+  const int64_t work = (int64_t)a.P.n_seq * a.max_q == a.P.n_tok
+                           ? a.P.n_seq * (((int64_t)a.max_q * a.gqa + bm - 1) / bm)
+                           : rows / bm + longest;
   const int64_t seen = a.window ? std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + bm / a.gqa + 1) : a.max_kv;
   const int64_t tiles = seen / kPT + 2;
-  // two workgroups fill a CU
-  const int64_t ns = std::min<int64_t>(2 * 256 / full, tiles / kMinTiles);
+  // As many splits as run at once, two workgroups a CU (head dim 512: one); one
+  // more is a second turn (6 chunks of up to 300 tokens under a window: 5 splits
+  // 45 us, 6 55).  Sequences of few rows beside them take up to half of the
+  // places (a prompt of 512 tokens at 2000 positions beside 60 tokens at up to
+  // 4000: f16 120 us with 14 splits, 101 with 7; 4 bits 82 and 63), but not
+  // so many that a workgroup has more than 64 tiles and outlasts them (2 x 1024
+  // tokens at 4096 beside 120: 4 bits 268 us with 1 split, 156 with 3).
+  const int64_t places = hd == 512 ? 256 : 512, units_of = std::max<int64_t>(1, work * a.P.kvh);
+  const int64_t beside = a.few_rows ? std::min<int64_t>(places / 2, 4 * (a.P.n_seq - longest) * a.P.kvh) : 0;
+  const int64_t fit = std::max((places - beside) / units_of, std::min((tiles + 63) / 64, places / units_of));
+  const int64_t ns = std::min<int64_t>(fit, tiles / kMinTiles);
   a.ns = (int)std::max<int64_t>(1, std::min<int64_t>(ns, 64));
   a.part_floats = a.ns > 1 ? (size_t)units * a.ns * bm * hd : 0;
   a.ml_floats = a.ns > 1 ? (size_t)units * a.ns * bm * 2 : 0;

@@ -3,10 +3,10 @@
 // merges in another.  One behind the other, decoded tokens waited for the
 // prompts beside them.  Head dim 256, 2 KV heads of 4 query heads, two launches
 // of each kind and these: a prompt of 512 tokens and 30 tokens at up to 2000
-// positions, f16 51 and 37 us, 4 bits 55 and 40; 2 chunks of 1024 tokens and 120
-// tokens at up to 4000, f16 252 and 207; 6 chunks alone, 4 bits, 107 and 89.
-// Head dim 128, 8 KV heads, 200 tokens and a chunk, 4 bits: 164 and 187, as
-// the tokens' workgroups have the chunks' registers here, two on a CU.
+// positions, f16 51 and 33 us, 4 bits 55 and 35; 2 chunks of 1024 tokens and 120
+// tokens at up to 4000, f16 252 and 205; 6 chunks alone, 4 bits, 107 and 80.
+// Head dim 128, 8 KV heads, 200 tokens and a chunk of 256, 4 bits: 164 and 160
+// (the tokens' workgroups have the chunks' registers here, two on a CU).
 #include "paged_chunk.h"
 #include "paged_few.h"
 
